@@ -301,6 +301,53 @@ int dgg_attn_decode_noalloc(const void* q, const void* k, const void* v, void* o
                             int64_t Hkv, int64_t L, int64_t D, const int64_t* strides, int64_t splits, float scale,
                             int dtype, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * A paged key/value cache: the serving form of the caches above, with a length per sequence. No counterpart in the
+ * reference, whose decode cases read one contiguous cache of one length.
+ *
+ * The cache is a pool of num_pages pages of page_size rows, k_pages / v_pages with element strides {page, row, head}
+ * and unit head-dim stride ([pages, page_size, Hkv, D] and [pages, Hkv, page_size, D] alike). Key j of sequence b is row
+ * j % page_size of page block_table[b][j / page_size] (int32, table_width entries a row).
+ * A step's T tokens are those of the B sequences one after the other: Sq tokens each (Sq > 0, cu_q NULL; T = B * Sq), or
+ * tokens [cu_q[b], cu_q[b+1]) (Sq = 0; cu_q int32 [B + 1], ascending from 0; rows from cu_q[B] on are not touched).
+ * kv_lens int32 [B]: the keys of each sequence, this step's included. The lengths and the table stay on the device:
+ * captured calls read them anew at every replay. Token tensors have strides {batch, token, head}; with cu_q the batch
+ * stride is not used and tokens are numbered through.
+ * ------------------------------------------------------------------------------------------- */
+
+/* Stores the step's keys and values: token i of sequence b, at position pos = kv_lens[b] - n_b + i, goes to row
+ * pos % page_size of its page. With rope_theta > 0 the key is rotated on the way (pairs (j, j + D/2) by the angle
+ * pos * rope_theta^(-2j/D), taken in 64 bits; rounded once, to the dtype), and so is the query row, if Hq > 0, from q to
+ * q_out (which may be q). rope_theta 0: no rotation, and no query (Hq 0). A token whose position lies outside the table's
+ * row, or whose page number outside [0, num_pages), is not stored. f32, f16, bf16; D a multiple of 16 up to 512; any
+ * page_size up to 2^20. strides: 19 int64 = q{b,t,h}, k{b,t,h}, v{b,t,h}, q_out{b,t,h}, k_pages{p,r,h}, v_pages{p,r,h},
+ * block_table{row}; all but the last multiples of 16 bytes, pointers 16-byte aligned. Two tokens of a call must not share
+ * a place. */
+int dgg_paged_append(const void* q, const void* k, const void* v, void* q_out, void* k_pages, void* v_pages,
+                     const int32_t* block_table, const int32_t* kv_lens, const int32_t* cu_q, int64_t B, int64_t T,
+                     int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D, int64_t num_pages, int64_t page_size,
+                     int64_t table_width, const int64_t* strides, float rope_theta, int dtype, void* stream);
+
+/* Attention of the step's queries over their sequences' pages: semantics of dgg_attn_prefill with Sq = n_b and
+ * Sk = kv_lens[b] (bottom-right causal mask, window, soft-cap, grouped heads) for each sequence, in one ragged launch, for
+ * decode rows, drafted tokens and prompt chunks alike. kv_lens beyond table_width * page_size is taken as that. Keys on a
+ * page number outside [0, num_pages) are not seen; what memory holds behind a sequence's last key or before its window
+ * does not matter. A row that sees no key gets o = 0 and lse = -inf (a padded sequence of a captured batch).
+ * prefix_len > 0 (whole pages): the first prefix_len keys of every sequence are those of sequence 0, read once for the
+ * whole batch through its row of the table, whatever the other rows say there; kv_lens include them.
+ * lse (optional): fp32 [T, Hq], natural logarithm. strides: 13 int64 = q{b,t,h}, k_pages{p,r,h}, v_pages{p,r,h}, o{b,t,h},
+ * block_table{row}; multiples of 8 elements but for the last. f16 / bf16, D in {64, 128, 256}, page_size a multiple of
+ * 16, B <= 4096; flags: DGG_ATTN_CAUSAL or 0. workspace: dgg_attn_paged_workspace_bytes(...) bytes, 16-byte aligned (no
+ * need to clear it; calls that overlap need one each). */
+int64_t dgg_attn_paged_workspace_bytes(int64_t B, int64_t T, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D,
+                                       int64_t prefix_len);
+int dgg_attn_paged(const void* q, const void* k_pages, const void* v_pages, void* o, float* lse,
+                   const int32_t* block_table, const int32_t* kv_lens, const int32_t* cu_q, void* workspace,
+                   int64_t workspace_bytes, int64_t B, int64_t T, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D,
+                   int64_t num_pages, int64_t page_size, int64_t table_width, int64_t prefix_len,
+                   const int64_t* strides, float scale, float softcap, int64_t window, uint32_t flags, int dtype,
+                   void* stream);
+
 /* Shader-clock probe (no counterpart in the reference: measurement support for the benchmark). One lane spins for
  * `ticks` ticks of the constant 100 MHz real-time counter and writes out[0] = shader cycles elapsed (s_memtime),
  * out[1] = real-time ticks elapsed: the shader clock is out[0] / out[1] * 100 MHz. out: 2 device uint64, 8-byte
