@@ -22,7 +22,7 @@
 
 namespace dgg_paged {
 
-constexpr int kTile = 32;     // keys per tile of the division
+constexpr int kTile = 128;    // keys per tile of the division
 constexpr int kGranule = 16;  // keys that are sure to lie in one page, one after another
 
 struct PagedParams {
@@ -46,7 +46,8 @@ struct PagedParams {
   int P;                    // shared prefix (a multiple of the page size)
   int causal, window;
   int R, rows_stride;       // rows per row group; rows of a partial (those that can be live)
-  int target, min_slice;    // units wanted over all KV heads, least tiles of a slice
+  int min_slice;            // least tiles of a slice
+  float per_target;         // (1 + 2^-11) Hkv / target: tiles of a unit, of all tiles of a KV head
   int grid_units, slots;
   dgg_attn::AttnParams s;   // scale and soft-cap constants (score_value)
 };
@@ -76,32 +77,37 @@ __device__ __forceinline__ int first_key(const PagedParams& p, const Seq& s) {
 }
 __device__ __forceinline__ int key_tiles(int lo, int hi) { return hi > lo ? (hi + kTile - 1) / kTile - lo / kTile : 0; }
 
-// Sums and inclusive prefix sums over a wave.
-__device__ __forceinline__ int64_t wave_sum64(int64_t x) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor((long long)x, off, 64);
+// Sums, extremes and inclusive prefix sums over a wave, on the DPP lane shifts (a sixth of the latency of ds_bpermute).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_or(int old, int x) {
+  return __builtin_amdgcn_update_dpp(old, x, CTRL, ROWS, 0xf, false);
+}
+// op over lanes 0 .. l in lane l; `none` leaves the other operand as it is.
+template <typename F>
+__device__ __forceinline__ int wave_scan(int x, int none, F op) {
+  x = op(x, dpp_or<0x111, 0xf>(none, x));  // row_shr:1
+  x = op(x, dpp_or<0x112, 0xf>(none, x));  // row_shr:2
+  x = op(x, dpp_or<0x114, 0xf>(none, x));  // row_shr:4
+  x = op(x, dpp_or<0x118, 0xf>(none, x));  // row_shr:8
+  x = op(x, dpp_or<0x142, 0xa>(none, x));  // row_bcast:15 into rows 1 and 3
+  x = op(x, dpp_or<0x143, 0xc>(none, x));  // row_bcast:31 into rows 2 and 3
   return x;
+}
+__device__ __forceinline__ int last_lane(int x) { return __builtin_amdgcn_readlane(x, 63); }
+__device__ __forceinline__ int wave_scan_add(int x) {
+  return wave_scan(x, 0, [](int a, int b) { return a + b; });
 }
 __device__ __forceinline__ int wave_min_i(int x) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) x = min(x, __shfl_xor(x, off, 64));
-  return x;
+  return last_lane(wave_scan(x, 0x7fffffff, [](int a, int b) { return min(a, b); }));
 }
 __device__ __forceinline__ int wave_max_i(int x) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) x = max(x, __shfl_xor(x, off, 64));
-  return x;
+  return last_lane(wave_scan(x, (int)0x80000000, [](int a, int b) { return max(a, b); }));
 }
-__device__ __forceinline__ int wave_scan(int x, int lane) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(x, off, 64);
-    if (lane >= off) x += y;
-  }
-  return x;
+__device__ __forceinline__ float wave_sum_f(float x) {
+  return __int_as_float(last_lane(wave_scan(__float_as_int(x), 0, [](int a, int b) {
+    return __float_as_int(__int_as_float(a) + __int_as_float(b));
+  })));
 }
-// Sum up to 2^31 - 1.
-__device__ __forceinline__ int wave_total(int x) { return (int)wave_sum64(x); }
 
 // What the whole wave knows after a look at all lengths.
 struct Division {
@@ -124,16 +130,16 @@ __device__ __forceinline__ int slices_of(const PagedParams& p, const Seq& s, int
 
 __device__ __forceinline__ Division divide(const PagedParams& p, int lane) {
   const int c = (p.B + 63) >> 6;
-  int64_t work = 0;
+  float work = 0.f;  // (32 bits do: the quotient is rounded up, and every wave adds in the same order)
   int lo = p.P;
   for (int j = 0; j < c; ++j) {
     const int b = lane * c + j;
     if (b >= p.B) break;
     const Seq s = load_seq(p, b);
-    work += (int64_t)row_groups(p, s) * key_tiles(first_key(p, s), s.kv);
+    work += (float)row_groups(p, s) * (float)key_tiles(first_key(p, s), s.kv);
     if (s.n > 0) lo = min(lo, p.window > 0 ? max(0, s.kv - s.n - p.window + 1) : 0);
   }
-  work = wave_sum64(work);
+  work = wave_sum_f(work);
   Division d;
   d.p_lo = 0;
   d.p_rg = d.p_ns = 0;
@@ -142,11 +148,11 @@ __device__ __forceinline__ Division divide(const PagedParams& p, int lane) {
     d.p_lo = wave_min_i(lo);
     d.p_rg = (p.T * p.G + p.R - 1) / p.R;
     p_tiles = key_tiles(d.p_lo, p.P);
-    work += (int64_t)d.p_rg * p_tiles;
+    work += (float)d.p_rg * (float)p_tiles;
   }
-  // (target >= Hkv; work * Hkv / target, rounded up)
-  const int64_t per = (work * p.Hkv + p.target - 1) / p.target;
-  d.slice = max(p.min_slice, (int)min(per, (int64_t)1 << 30));
+  // At least work * Hkv / target: the sum of 4096 terms in fp32 is off by less than 2^-12 of it.
+  const float per = work * p.per_target;
+  d.slice = max(p.min_slice, (int)ceilf(min(per, 1e9f)));
   if (p.P > 0) d.p_ns = ceil_div(p_tiles, d.slice);
   return d;
 }
@@ -177,11 +183,11 @@ __device__ __forceinline__ Place find_place(const PagedParams& p, const Division
   }
   Place r{};
   r.b = -1;
-  int incl = wave_scan(mine, lane), sincl = wave_scan(my_slots, lane);
+  int incl = wave_scan_add(mine), sincl = wave_scan_add(my_slots);
   unsigned long long hit = __ballot(u < incl);
   if (hit == 0) return r;
   int at = __ffsll(hit) - 1;
-  int base = __shfl(incl - mine, at, 64), sbase = __shfl(sincl - my_slots, at, 64);
+  int base = __builtin_amdgcn_readlane(incl - mine, at), sbase = __builtin_amdgcn_readlane(sincl - my_slots, at);
   r.b = at;
   if (c > 1) {  // lane j looks at the j-th of that lane's sequences (c <= 64: B <= 4096)
     const int b = at * c + lane;
@@ -190,8 +196,8 @@ __device__ __forceinline__ Place find_place(const PagedParams& p, const Division
       s0 = load_seq(p, b);
       mine = count(s0, ns0, my_slots);
     }
-    incl = wave_scan(mine, lane);
-    sincl = wave_scan(my_slots, lane);
+    incl = wave_scan_add(mine);
+    sincl = wave_scan_add(my_slots);
     hit = __ballot(u - base < incl);
     if (hit == 0) {  // (cannot be: the lane's sum exceeds u - base)
       r.b = -1;
@@ -200,16 +206,15 @@ __device__ __forceinline__ Place find_place(const PagedParams& p, const Division
     r.b = at * c;
     at = __ffsll(hit) - 1;
     r.b += at;
-    base += __shfl(incl - mine, at, 64);
-    sbase += __shfl(sincl - my_slots, at, 64);
+    base += __builtin_amdgcn_readlane(incl - mine, at);
+    sbase += __builtin_amdgcn_readlane(sincl - my_slots, at);
   }
-  r.b = __builtin_amdgcn_readfirstlane(r.b);
-  r.s.t0 = __builtin_amdgcn_readfirstlane(__shfl(s0.t0, at, 64));
-  r.s.n = __builtin_amdgcn_readfirstlane(__shfl(s0.n, at, 64));
-  r.s.kv = __builtin_amdgcn_readfirstlane(__shfl(s0.kv, at, 64));
-  r.ns = __builtin_amdgcn_readfirstlane(__shfl(ns0, at, 64));
-  r.local = __builtin_amdgcn_readfirstlane(u - base);
-  r.slot = __builtin_amdgcn_readfirstlane(sbase);
+  r.s.t0 = __builtin_amdgcn_readlane(s0.t0, at);
+  r.s.n = __builtin_amdgcn_readlane(s0.n, at);
+  r.s.kv = __builtin_amdgcn_readlane(s0.kv, at);
+  r.ns = __builtin_amdgcn_readlane(ns0, at);
+  r.local = u - base;
+  r.slot = sbase;
   return r;
 }
 

@@ -1,18 +1,21 @@
-// Attention over a paged key/value cache (dgg_attn_paged): decode rows, drafted tokens and prompt chunks of a ragged batch
-// in one launch, optionally behind a prefix that all sequences share. paged.h has the division of the work.
+// Attention over a paged key/value cache (dgg_attn_paged): decode rows, drafted tokens and prompt chunks of a ragged
+// batch in one launch, optionally behind a prefix that all sequences share. paged.h has the division of the work.
 //
 //   scores = cap(q . k^T * scale), masked; p = softmax(scores); o = p . v
 //
-// Each unit is a workgroup of NW waves with 32 rows each over one slice of the keys, in tiles of 32: K and V rows go
-// global -> registers -> LDS one tile ahead of the compute, then
+// in tiles of keys that go straight from the pages to the LDS (global_load_lds, DmaLayout of attention_common.h):
 //   S^T (32 keys x 32 rows) = K . Q^T     v_mfma_f32_32x32x16, A = K from the LDS, B = Q in registers
 //   O^T (D x 32 rows)      += V^T . P^T   A = V^T by transposing LDS reads, B = P from the S^T accumulator
 // with one running maximum and sum per row, in fp32; P is rounded to the storage type, as the matrix instruction takes it
-// (its error is that of the output's own rounding, spread over the keys). Partials of split rows are merged by a second
-// kernel.
+// (its error is that of the output's own rounding, spread over the keys). Two kernels:
+//   narrow  up to 32 rows of a KV head: bound by the stream of keys and values. Four waves share the rows and take the
+//           32-key tiles in turn, each with buffers of its own and no barrier, and add their states at the end;
+//   wide    more rows: bound by the matrix products. The waves share the tiles and have rows of their own.
+// Partials of split rows are joined by a third.
 //
-// Keys that no row of the sequence may see (behind kv_len, before the window, on a page number outside the pool) are never
-// multiplied: their rows are replaced by a visible key's, so what memory holds there does not matter.
+// A granule is 16 keys, which lie in one page one after another. Granules that hold no key of the unit (behind kv_len,
+// before the window, on a page number outside the pool) are zeros in the LDS and masked; rows of a granule that are no
+// keys are replaced by one that is. What memory holds there does not matter.
 #include <climits>
 
 #include "common.h"
@@ -25,381 +28,791 @@ namespace {
 using namespace dgg_attn;
 using namespace dgg_paged;
 
-// Registers: two waves per SIMD at head_dim 64 and 128, one at 256 (Q 64 + O 128 registers).
-template <typename T, int D, int NW, bool SOFTCAP>
-__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D >= 256 ? 1 : 2)))
-paged_attn_kernel(PagedParams p) {
+// The unit of this workgroup and its keys.
+struct Unit {
+  bool prefix;
+  int b;          // sequence (prefix: 0, whose table it reads)
+  Seq s;
+  int row0, rows; // first row; rows of the row space (the sequence's, or the whole batch's)
+  int slot;       // partial slot, or -1: the unit writes the output
+  int lo, hi;     // keys of it that any row of the row group sees
+  int k0, k1;     // keys of the slice (k0 a multiple of kTile); those of [lo, hi) count
+};
+__device__ __forceinline__ bool find_unit(const PagedParams& p, int lane, Unit& u) {
+  const Division dv = divide(p, lane);
+  const int p_units = dv.p_rg * dv.p_ns;
+  const int bid = blockIdx.x;
+  u.prefix = bid < p_units;
+  int k, ns;
+  if (u.prefix) {
+    k = bid / dv.p_rg;
+    const int rg = bid - k * dv.p_rg;
+    ns = dv.p_ns;
+    u.b = 0;
+    u.row0 = rg * p.R;
+    u.rows = p.T * p.G;
+    u.slot = rg * dv.p_ns + k;
+    u.lo = dv.p_lo;
+    u.hi = p.P;
+  } else {
+    const Place pl = find_place<true>(p, dv, bid - p_units, lane);
+    if (pl.b < 0) return false;
+    const int nrg = row_groups(p, pl.s);
+    k = pl.local / nrg;
+    const int rg = pl.local - k * nrg;
+    ns = pl.ns;
+    u.b = pl.b;
+    u.s = pl.s;
+    u.row0 = rg * p.R;
+    u.rows = pl.s.n * p.G;
+    u.slot = p.P > 0 || pl.ns > 1 ? p_units + pl.slot + rg * pl.ns + k : -1;
+    const int off = pl.s.kv - pl.s.n;
+    u.lo = first_key(p, pl.s);
+    u.hi = pl.s.kv;
+    if (p.causal) u.hi = min(u.hi, (min(u.row0 + p.R, u.rows) - 1) / p.G + off + 1);
+    if (p.window > 0) u.lo = max(u.lo, u.row0 / p.G + off - p.window + 1);
+  }
+  const int tiles = key_tiles(u.lo, u.hi), per = ceil_div(tiles, ns), t0 = u.lo / kTile;
+  u.k0 = (t0 + min(tiles, k * per)) * kTile;
+  u.k1 = (t0 + min(tiles, (k + 1) * per)) * kTile;
+  return true;
+}
+
+// A query row of the unit, as a lane holds it.
+struct Row {
+  bool ok;
+  int tok, h;       // token, query head
+  int64_t q, o;     // element offsets of the row in q and o
+  int k_lo, k_hi;   // keys it sees: k_lo <= key <= k_hi
+};
+__device__ __forceinline__ Row find_row(const PagedParams& p, const Unit& u, int rl, int hk) {
+  Row x{};
+  const int row = u.row0 + rl;
+  x.ok = row < u.rows && rl < p.R;
+  int i = 0, b = u.b;
+  Seq s = u.s;
+  if (x.ok) {
+    i = row / p.G;
+    x.h = hk * p.G + (row - i * p.G);
+    if (u.prefix) {
+      x.tok = i;
+      b = seq_of_token(p, i);
+      x.ok = b < p.B;
+      if (x.ok) {
+        s = load_seq(p, b);
+        i -= s.t0;
+        x.ok = i >= 0 && i < s.n;
+      }
+    } else {
+      x.tok = s.t0 + i;
+    }
+  }
+  if (!x.ok) return Row{false, 0, 0, 0, 0, 0, -1};
+  x.q = (p.cu_q != nullptr ? x.tok * p.q_ss : b * p.q_sb + i * p.q_ss) + x.h * p.q_sh;
+  x.o = (p.cu_q != nullptr ? x.tok * p.o_ss : b * p.o_sb + i * p.o_ss) + x.h * p.o_sh;
+  x.k_hi = min(u.hi, s.kv) - 1;
+  x.k_lo = u.lo;
+  if (p.causal) x.k_hi = min(x.k_hi, i + s.kv - s.n);
+  if (p.window > 0) x.k_lo = max(x.k_lo, i + s.kv - s.n - p.window + 1);
+  return x;
+}
+
+// What the rows of a wave see together: a block of keys inside [lo_max, hi_min] is seen whole by every row (a row that
+// sees no key makes every block masked; lanes without a row do not count), one outside [lo_min, hi_max] by none.
+struct Seen {
+  int lo_max, hi_min, lo_min, hi_max;
+};
+__device__ __forceinline__ Seen seen_by_wave(const Row& x) {
+  const bool empty = x.k_hi < x.k_lo;
+  Seen v;
+  v.lo_max = __any(x.ok) ? wave_max_i(!x.ok ? INT_MIN : empty ? INT_MAX : x.k_lo) : INT_MAX;
+  v.hi_min = wave_min_i(!x.ok ? INT_MAX : empty ? INT_MIN : x.k_hi);
+  v.lo_min = wave_min_i(x.ok && !empty ? x.k_lo : INT_MAX);
+  v.hi_max = wave_max_i(x.ok && !empty ? x.k_hi : INT_MIN);
+  return v;
+}
+
+// Where 64 granules are, one per lane: byte offsets of their first K and V row, and which of them hold a key of the unit.
+// The page numbers of the next 64 are requested when these are taken up, so that their latency is not waited for.
+struct Granules {
+  const int32_t* row;  // the sequence's row of the table
+  int64_t ko, vo;
+  int next;            // page number of the granule that comes next
+  uint64_t live;       // bit l: the granule of lane l holds a key
+  __device__ __forceinline__ int page_of(const PagedParams& p, int gi) {
+    return row[min(gi, p.cap / kGranule - 1) / p.gpp];
+  }
+  // Takes up granule gi (per lane) with its page number in `next`, and requests that of gi_next.
+  __device__ __forceinline__ void take(const PagedParams& p, const Unit& u, int gi, int gi_next) {
+    const int page = next;
+    next = page_of(p, gi_next);
+    const int key = gi * kGranule;
+    const bool ok = page >= 0 && page < p.num_pages && key + kGranule > u.lo && key < min(u.hi, u.k1);
+    const int in = (gi % p.gpp) * kGranule;
+    ko = 2 * (page * p.k_sp + in * p.k_ss);
+    vo = 2 * (page * p.v_sp + in * p.v_ss);
+    live = __ballot(ok);
+  }
+};
+__device__ __forceinline__ int64_t lane64(int64_t x, int at) {
+  const unsigned lo32 = __builtin_amdgcn_readlane((int)(x & 0xffffffff), at);
+  const int hi32 = __builtin_amdgcn_readlane((int)(x >> 32), at);
+  return (int64_t)hi32 << 32 | lo32;
+}
+
+// Copies one granule (16 rows of D) of K or V to `lds`, the place of its first 4- or 8-row group. kWhole: every row is a
+// key. Otherwise rows outside [first, last] are replaced by the nearest that is inside.
+template <int D>
+struct GranuleCopy {
+  typedef DmaLayout<D> L;
+  static constexpr int LOADS = kGranule / L::RPI;  // direct loads per granule
+  uint32_t voff[L::NV];  // lane constants: row within the load's group, and the chunk that the layout puts there
+  uint32_t chunk[L::NV];
+  int lrow;
+  // D == 64: the swizzle depends on the 8-row group's number, whose parity is that of the load within the granule.
+  static __device__ __forceinline__ int vi(int i) { return D == 64 ? i & 1 : i % L::IPG; }
+  __device__ __forceinline__ void init(int lane, int64_t ss_b) {
+    lrow = lane / L::LPR;
+#pragma unroll
+    for (int i = 0; i < L::NV; ++i) {
+      const int trow = i * L::RPI + lrow;  // (row within a granule, which is all that the swizzle looks at)
+      chunk[i] = (uint32_t)((lane % L::LPR) ^ L::swizzle(trow)) * 16u;
+      voff[i] = (uint32_t)((D == 64 ? lrow : trow) * ss_b) + chunk[i];
+      asm volatile("" : "+v"(voff[i]));
+    }
+  }
+  static __device__ __forceinline__ uint32_t place(int i) {
+    return (uint32_t)((i / L::IPG) * L::GROUP_B + (i % L::IPG) * L::RPI * L::ROW_B);
+  }
+  __device__ __forceinline__ void one(uint32_t lds, const char* base, int64_t ss_b, int i) const {
+    dma16(lds + place(i), base + (int64_t)(D == 64 ? i * L::RPI : (i / L::IPG) * L::GR) * ss_b, voff[vi(i)]);
+  }
+  __device__ __forceinline__ void whole(uint32_t lds, const char* base, int64_t ss_b) const {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) one(lds, base, ss_b, i);
+  }
+  __device__ __forceinline__ void part(uint32_t lds, const char* base, int64_t ss_b, int first, int last) const {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int row = clampi(i * L::RPI + lrow, first, last);
+      dma16(lds + place(i), base + (row * ss_b + chunk[vi(i)]));
+    }
+  }
+  static __device__ __forceinline__ void zero(uint32_t lds, int lane) {
+    typedef float __attribute__((ext_vector_type(4))) f4;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+      *reinterpret_cast<f4 __attribute__((address_space(3)))*>((lds_char*)(size_t)(lds + place(i) + 16 * lane)) = f4{};
+  }
+};
+
+// LDS addresses of a tile's fragments, per lane. K fragment kk of the 32-key block at row 0: k[ki(kk)] + ko(kk). V
+// transposing read of keys 16kk + 4g + .. (hi: + 8), head-dim block db: v[vb(db, hi)] + vo(kk, hi).
+template <int D>
+struct Fragments {
+  typedef DmaLayout<D> L;
+  static constexpr int NK = D == 64 ? D / 16 : D / 32, NV = D == 64 ? 2 * (D / 32) : D / 32;
+  uint32_t k[NK], v[NV];
+  static constexpr int ki(int kk) { return D == 64 ? kk : kk >> 1; }
+  static constexpr int ko(int mb, int kk) { return mb * (32 / L::GR) * L::GROUP_B + (D == 64 ? 0 : 32 * (kk & 1)); }
+  static constexpr int vb(int db, int hi) { return D == 64 ? 2 * db + hi : db; }
+  static constexpr int vo(int kk, int hi) { return kk * (16 / L::GR) * L::GROUP_B + hi * (8 / L::GR) * L::GROUP_B; }
+  // k_at, v_at: where the tile's K and V rows begin
+  __device__ __forceinline__ void init(int lane, uint32_t k_at, uint32_t v_at) {
+    const int r = lane & 31, g = lane >> 5, m4 = (lane & 15) >> 2, m3 = lane & 3;
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      const int chunk = D == 64 ? 2 * i + g : 4 * i;  // (D >= 128: g and kk & 1 do not meet the swizzled bits)
+      k[i] = k_at + (uint32_t)((r / L::GR) * L::GROUP_B + (r % L::GR) * L::ROW_B + 16 * (chunk ^ L::swizzle(r)) +
+                               (D == 64 ? 0 : 16 * g));
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int row = 4 * g + m4 + (D == 64 ? 8 * (i & 1) : 0);  // hi reads of D == 64 swizzle differently
+      const int chunk = 4 * (D == 64 ? i >> 1 : i) + 2 * ((lane >> 4) & 1) + (m3 >> 1);
+      v[i] = v_at + (uint32_t)(((row & 7) / L::GR) * L::GROUP_B + (row % L::GR) * L::ROW_B +
+                               16 * (chunk ^ L::swizzle(row)) + 8 * (m3 & 1));
+    }
+  }
+};
+
+// Running softmax state of a wave's 32 rows (lanes r and r + 32 share row r).
+template <int D>
+struct State {
+  f32x16 o[D / 32];
+  float m;      // reference maximum (value units)
+  float l[2];   // sums of this lane's probabilities
+  __device__ __forceinline__ void init() {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) o[i] = f32x16{};
+    m = -INFINITY;
+    l[0] = l[1] = 0.f;
+  }
+  // Raises the maximum where mloc exceeds it by enough to matter.
+  __device__ __forceinline__ void raise(float mloc, float c) {
+    mloc = half_swap_max(mloc);
+    const float m_new = fmaxf(m, mloc);
+    const bool need = m_new * c > m * c + kRescaleThreshold;
+    if (__any(need)) {
+      const float alpha = need ? fast_exp2((m - m_new) * c) : 1.0f;
+      if (need) m = m_new;
+      l[0] *= alpha;
+      l[1] *= alpha;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) o[i] *= alpha;
+    }
+  }
+};
+
+constexpr int kOQ = 64 * 16 + 16;  // a quad of O registers of a wave in the LDS, and padding
+
+// Leaves a wave's state in its slot: D / 8 quads of O, and (maximum in the exp2 domain, sum) of each row.
+template <int D>
+__device__ __forceinline__ void put_state(const State<D>& st, char* slot, f32x2* ml, float c, int lane) {
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int jj = 0; jj < 4; ++jj)
+      *reinterpret_cast<f32x4*>(slot + (db * 4 + jj) * kOQ + lane * 16) =
+          f32x4{st.o[db][4 * jj], st.o[db][4 * jj + 1], st.o[db][4 * jj + 2], st.o[db][4 * jj + 3]};
+  const float l = half_swap_sum(st.l[0] + st.l[1]);
+  if (lane < 32) ml[lane] = f32x2{st.m == -INFINITY ? -INFINITY : st.m * c, l};
+}
+
+// Joins KG states (slot i * step) of a row and writes 8 of its head-dim elements: the output, or a partial of the unit.
+template <typename T, int D, int KG>
+__device__ __forceinline__ void write_row(const PagedParams& p, const Unit& u, const char* slots, const f32x2* ml, int step,
+                                          int slot_b, int r, int quad, int64_t o_off, int64_t tok_h, int rl, int hk) {
+  typedef typename T::scalar S;
+  typedef typename T::vec8 V8;
+  float wt[KG], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < KG; ++i) m = fmaxf(m, ml[i * step * 32 + r][0]);
+  const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+  for (int i = 0; i < KG; ++i) {
+    const f32x2 x = ml[i * step * 32 + r];
+    wt[i] = fast_exp2(x[0] - mu);
+    l = fmaf(wt[i], x[1], l);
+  }
+  f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+#pragma unroll
+  for (int i = 0; i < KG; ++i) {
+    const char* s = slots + (int64_t)i * step * slot_b + quad * kOQ + r * 16;
+    lo += wt[i] * *reinterpret_cast<const f32x4*>(s);
+    hi += wt[i] * *reinterpret_cast<const f32x4*>(s + 32 * 16);
+  }
+  if (u.slot < 0) {
+    const float inv = l == 0.f ? 0.f : 1.0f / l;  // a row that sees no key: o = 0, lse = -inf
+    st16(static_cast<S*>(p.o) + o_off + 8 * quad,
+         from_f32x8<V8>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7) * inv));
+    if (p.lse != nullptr && quad == 0) p.lse[tok_h] = l == 0.f ? -INFINITY : (m + fast_log2(l)) * kLn2;
+    return;
+  }
+  if (u.slot >= p.slots) return;  // (only where cu_q descends)
+  const int64_t x = ((int64_t)u.slot * p.Hkv + hk) * p.rows_stride + rl;
+  *reinterpret_cast<f32x4*>(p.part_o + x * D + 8 * quad) = lo;
+  *reinterpret_cast<f32x4*>(p.part_o + x * D + 8 * quad + 4) = hi;
+  if (quad == 0) *reinterpret_cast<f32x2*>(p.part_ml + 2 * x) = f32x2{m, l};
+}
+
+// Scores of one 32-key block in the exp2 domain's value units, masked where `masked`; returns their maximum.
+template <typename T, bool SOFTCAP, bool MASKED>
+__device__ __forceinline__ float block_scores(f32x16& s, const PagedParams& p, int rel_lo, int rel_hi, unsigned holes) {
+  float mloc = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {  // element j holds key 8*(j/4) + 4g + j%4 of the block (rel_*: less 4g)
+    float x = score_value<T, SOFTCAP, 0>(s[j], p.s);
+    if constexpr (MASKED) {
+      const int o = 8 * (j >> 2) + (j & 3);
+      x = (o <= rel_hi && o >= rel_lo && !(holes & (j < 8 ? 1u : 2u))) ? x : -INFINITY;
+    }
+    s[j] = x;
+    mloc = fmaxf(mloc, x);
+  }
+  return mloc;
+}
+
+constexpr int kNarrowWaves = 4;
+
+// Waves per SIMD: as many workgroups per CU as the LDS holds (33 KiB at head_dim 64, 67 at 128, 133 at 256).
+template <typename T, int D, bool SOFTCAP>
+__global__ void __launch_bounds__(64 * kNarrowWaves)
+__attribute__((amdgpu_waves_per_eu(D >= 256 ? 1 : D >= 128 ? 2 : 4))) paged_narrow_kernel(PagedParams p) {
+  typedef DmaLayout<D> L;
   typedef typename T::scalar S;
   typedef typename T::vec8 V8;
   typedef typename T::vec4 V4;
-  constexpr int BN = kTile;
-  constexpr int KP = D + 8;             // padded row (elements): 16-byte shift per row for both read patterns
-  constexpr int NKK = D / 16;           // MFMA k-steps over the head dim
-  constexpr int NDB = D / 32;           // 32-wide head-dim blocks of O^T
-  constexpr int NPK = BN / 16;          // MFMA k-steps over the keys of a tile in P.V
-  constexpr int NT = 64 * NW;
-  constexpr int LPR = D / 8;            // threads per key row: consecutive lanes read consecutive 16-byte chunks
-  constexpr int RPI = NT / LPR;         // key rows per load instruction of the workgroup
-  constexpr int CPT = BN / RPI;         // 16-byte chunks per thread per tile (K and V each)
-  static_assert(CPT * RPI == BN && RPI * LPR == NT, "tile mapping");
-
-  __shared__ __attribute__((aligned(16))) S Ks[BN][KP];
-  __shared__ __attribute__((aligned(16))) S Vs[BN][KP];
+  constexpr int NW = kNarrowWaves;
+  constexpr int TILE_B = (32 / L::GR) * L::GROUP_B;  // K or V rows of 32 keys
+  constexpr int GRAN_B = (kGranule / L::GR) * L::GROUP_B;
+  constexpr int LOADS = 2 * GranuleCopy<D>::LOADS;   // direct loads of a tile, K or V
+  constexpr int WAVE_B = std::max(2 * TILE_B, (D / 8) * kOQ);
+  __shared__ __attribute__((aligned(1024))) char smem[NW * (WAVE_B + 32 * 8)];
 
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hk = blockIdx.y;
+  Unit u;
+  if (!find_unit(p, lane, u)) return;
 
-  // This workgroup's unit.
-  const Division dv = divide(p, lane);
-  const int p_units = dv.p_rg * dv.p_ns;
-  const bool prefix = (int)blockIdx.x < p_units;
-  Place pl{};
-  int row0, rows, slot, lo, hi, kslice, nslices;  // first row, rows (of the row space), keys of the row group
-  if (prefix) {
-    kslice = (int)blockIdx.x / dv.p_rg;
-    const int rg = (int)blockIdx.x - kslice * dv.p_rg;
-    nslices = dv.p_ns;
-    row0 = rg * p.R;
-    rows = p.T * p.G;
-    slot = rg * dv.p_ns + kslice;
-    lo = dv.p_lo;
-    hi = p.P;
-  } else {
-    pl = find_place<true>(p, dv, (int)blockIdx.x - p_units, lane);
-    if (pl.b < 0) return;
-    const int nrg = row_groups(p, pl.s);
-    kslice = pl.local / nrg;
-    const int rg = pl.local - kslice * nrg;
-    nslices = pl.ns;
-    row0 = rg * p.R;
-    rows = pl.s.n * p.G;
-    slot = p.P > 0 || pl.ns > 1 ? p_units + pl.slot + rg * pl.ns + kslice : -1;
-    // keys that any of these rows sees
-    const int off = pl.s.kv - pl.s.n;
-    lo = first_key(p, pl.s);
-    hi = pl.s.kv;
-    if (p.causal) hi = min(hi, (min(row0 + p.R, rows) - 1) / p.G + off + 1);
-    if (p.window > 0) lo = max(lo, row0 / p.G + off - p.window + 1);
+  // The wave's tiles: every NW-th of the slice's 32-key tiles that hold a key.
+  const int t_first = max(u.k0, u.lo) / 32, t_end = ceil_div(min(u.k1, u.hi), 32);
+  const int n_own = u.k1 > u.k0 ? max(0, ceil_div(t_end - t_first - w, NW)) : 0;
+  auto tile_of = [&](int s) { return t_first + w + NW * s; };
+  auto gran_of = [&](int s0) { return 2 * tile_of(s0 + (lane >> 1)) + (lane & 1); };
+  Granules gr;
+  gr.row = p.table + u.b * p.table_sb;
+  if (n_own > 0) gr.next = gr.page_of(p, gran_of(0));
+
+  const Row x = find_row(p, u, r, hk);
+  const S* qp = static_cast<const S*>(p.q) + x.q;
+  V8 qf[D / 16];
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) qf[kk] = ld16<V8>(qp + 16 * kk + 8 * g);
+
+  const uint32_t wave_at = (uint32_t)(size_t)((lds_char*)smem) + w * WAVE_B;
+  const int64_t k_ss_b = 2 * p.k_ss, v_ss_b = 2 * p.v_ss;
+  GranuleCopy<D> kc, vc;
+  kc.init(lane, k_ss_b);
+  vc.init(lane, v_ss_b);
+  Fragments<D> fr;
+  fr.init(lane, wave_at, wave_at + TILE_B);
+  const char* kp = static_cast<const char*>(p.k) + 2 * hk * p.k_sh;
+  const char* vp = static_cast<const char*>(p.v) + 2 * hk * p.v_sh;
+
+  // Copies the K (V) rows of own tile s to the wave's K (V) buffer.
+  const int end = min(u.hi, u.k1);
+  auto copy = [&](int s, bool values) {
+    const int64_t off = values ? gr.vo : gr.ko, ss_b = values ? v_ss_b : k_ss_b;
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const int at = 2 * (s & 31) + hh, key = tile_of(s) * 32 + hh * kGranule;
+      const uint32_t lds = wave_at + (values ? TILE_B : 0) + hh * GRAN_B;
+      const char* base = (values ? vp : kp) + lane64(off, at);
+      const GranuleCopy<D>& c = values ? vc : kc;
+      if (!((gr.live >> at) & 1)) c.zero(lds, lane);
+      else if (key >= u.lo && key + kGranule <= end) c.whole(lds, base, ss_b);
+      else c.part(lds, base, ss_b, max(0, u.lo - key), min(kGranule, end - key) - 1);
+    }
+  };
+  auto holes_of = [&](int s) { return ~(unsigned)(gr.live >> (2 * (s & 31))) & 3u; };
+
+  const Seen see = seen_by_wave(x);
+  State<D> st;
+  st.init();
+  const float c = score_coeff<SOFTCAP, 0>(p.s);
+  unsigned holes = 0;
+  if (n_own > 0) {
+    gr.take(p, u, gran_of(0), gran_of(32));
+    copy(0, false);
+    copy(0, true);
+    holes = holes_of(0);
   }
-  const int b_table = prefix ? 0 : pl.b;
-  const int tile0 = lo / BN, tiles = key_tiles(lo, hi), per = ceil_div(tiles, nslices);
-  const int t_begin = tile0 + min(tiles, kslice * per), t_end = tile0 + min(tiles, kslice * per + per);
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) {
+    asm volatile("" : "+v"(qf[kk]));
+    if (!x.ok) qf[kk] = V8{};
+  }
+  for (int s = 0; s < n_own; ++s) {
+    const int kt = tile_of(s) * 32;
+    const bool more = s + 1 < n_own;
+    const bool live = holes != 3 && kt <= see.hi_max && kt + 31 >= see.lo_min;
+    const bool full = holes == 0 && kt >= see.lo_max && kt + 31 <= see.hi_min;
+    // The K copies are the older half of what is outstanding (a hole's zeros are no copies: then wait for everything).
+    if (holes == 0) wait_vmem<LOADS>();
+    else wait_vmem<0>();
+    f32x16 sacc = f32x16{};
+    if (live) {
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+        sacc = mfma32(lds_read<V8>(fr.k[fr.ki(kk)] + fr.ko(0, kk)), qf[kk], sacc);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the K buffer is read
+    // The next K tile is requested before this one's softmax. (The values of a 32-tile window's last tile are copied
+    // before its offsets are given up: V of tile s + 1 below uses the window that K took up.)
+    unsigned next_holes = 0;
+    if (more) {
+      if (((s + 1) & 31) == 0) gr.take(p, u, gran_of(s + 1), gran_of(s + 33));
+      next_holes = holes_of(s + 1);
+      copy(s + 1, false);
+    }
+    if (live) {
+      const int k4 = kt + 4 * g;
+      const float mloc = full ? block_scores<T, SOFTCAP, false>(sacc, p, 0, 0, 0)
+                              : block_scores<T, SOFTCAP, true>(sacc, p, x.k_lo - k4, x.k_hi - k4, holes);
+      st.raise(mloc, c);
+    }
+    if (more && next_holes == 0) wait_vmem<LOADS>();
+    else wait_vmem<0>();
+    if (live) {
+      const float mc = st.m == -INFINITY ? 0.f : st.m * c;
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        f32x8 pv;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float pe = fast_exp2(fmaf(sacc[8 * kk + e], c, -mc));
+          st.l[e & 1] += pe;
+          pv[e] = pe;
+        }
+        const V8 pb = from_f32x8<V8>(pv);
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) {
+          const V4 a0 = tr_read_at(fr.v[fr.vb(db, 0)] + fr.vo(kk, 0), S{});
+          const V4 a1 = tr_read_at(fr.v[fr.vb(db, 1)] + fr.vo(kk, 1), S{});
+          st.o[db] = mfma32(__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7), pb, st.o[db]);
+        }
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the V buffer is read
+    if (more) copy(s + 1, true);
+    holes = next_holes;
+  }
 
-  // This lane's row (query column of S^T): lanes r and r + 32 share it.
-  const int rl = w * 32 + r;  // row within the row group
-  const int row = row0 + rl;
-  bool row_ok = row < rows;
-  int tok = 0, qi = 0, qg = 0, kv = 0, n = 0, b = 0;
-  if (row_ok) {
-    const int i = row / p.G;
-    qg = row - i * p.G;
-    if (prefix) {
-      tok = i;
-      b = seq_of_token(p, tok);
-      row_ok = b < p.B;
-      if (row_ok) {
-        const Seq s = load_seq(p, b);
-        qi = tok - s.t0;
-        n = s.n;
-        kv = s.kv;
-        row_ok = qi >= 0 && qi < n;
+  // The waves' states over disjoint keys are joined: O = sum_i 2^(m_i - m) O_i, l alike.
+  char* slots = smem;
+  f32x2* ml = reinterpret_cast<f32x2*>(smem + NW * WAVE_B);
+  wait_vmem<0>();
+  put_state(st, slots + w * WAVE_B, ml + 32 * w, c, lane);
+  __syncthreads();
+  const int live_rows = min(32, u.rows - u.row0);
+  for (int it = tid; it < live_rows * (D / 8); it += 64 * NW) {
+    const int row = it / (D / 8), quad = it % (D / 8);
+    const Row y = find_row(p, u, row, hk);
+    if (!y.ok) continue;
+    write_row<T, D, NW>(p, u, slots, ml, 1, WAVE_B, row, quad, y.o, (int64_t)y.tok * p.Hq + y.h, row, hk);
+  }
+}
+
+// NW waves over tiles of BN keys in a ring of two. KG: waves that share the same 32 rows, each taking BN / KG keys of every
+// tile; a workgroup covers 32 * NW / KG rows. Each wave copies one granule of a tile (BN = 16 NW).
+template <typename T, int D, int NW, int KG, int OCC, bool SOFTCAP>
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
+paged_wide_kernel(PagedParams p) {
+  typedef DmaLayout<D> L;
+  typedef typename T::scalar S;
+  typedef typename T::vec8 V8;
+  typedef typename T::vec4 V4;
+  constexpr int BN = kGranule * NW, SBN = BN / KG, NMB = SBN / 32, NWR = NW / KG;
+  constexpr int TILE_B = (BN / L::GR) * L::GROUP_B, STAGE_B = 2 * TILE_B;
+  constexpr int GRAN_B = (kGranule / L::GR) * L::GROUP_B;
+  constexpr int WINDOW = 64 / NW;                    // tiles whose granules the lanes hold
+  constexpr int SLOT_B = (D / 8) * kOQ;
+  constexpr int LOADS = GranuleCopy<D>::LOADS;
+  constexpr int SMEM_B = std::max(2 * STAGE_B, NW * (SLOT_B + 32 * 8));
+  static_assert(SBN % 32 == 0, "key groups");
+  __shared__ __attribute__((aligned(1024))) char smem[SMEM_B];
+
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = KG == 1 ? w : w % NWR, kg = KG == 1 ? 0 : w / NWR;
+  const int koff = SBN * kg;
+  const int hk = blockIdx.y;
+  Unit u;
+  if (!find_unit(p, lane, u)) return;
+
+  const int end = min(u.hi, u.k1);
+  const int t_first = max(u.k0, u.lo) / BN, t_end = u.k1 > u.k0 ? ceil_div(end, BN) : t_first;
+  auto gran_of = [&](int t0) { return NW * (t0 + lane / NW) + lane % NW; };
+  Granules gr;
+  gr.row = p.table + u.b * p.table_sb;
+  if (t_first < t_end) gr.next = gr.page_of(p, gran_of(t_first));
+
+  const int rl = 32 * wr + r;
+  const Row x = find_row(p, u, rl, hk);
+  const S* qp = static_cast<const S*>(p.q) + x.q;
+  V8 qf[D / 16];
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) qf[kk] = ld16<V8>(qp + 16 * kk + 8 * g);
+
+  const uint32_t smem_at = (uint32_t)(size_t)((lds_char*)smem);
+  const int64_t k_ss_b = 2 * p.k_ss, v_ss_b = 2 * p.v_ss;
+  GranuleCopy<D> kc, vc;
+  kc.init(lane, k_ss_b);
+  vc.init(lane, v_ss_b);
+  Fragments<D> fr;
+  fr.init(lane, smem_at + (koff / L::GR) * L::GROUP_B, smem_at + TILE_B + (koff / L::GR) * L::GROUP_B);
+  const char* kp = static_cast<const char*>(p.k) + 2 * hk * p.k_sh;
+  const char* vp = static_cast<const char*>(p.v) + 2 * hk * p.v_sh;
+
+  // The wave's granule of the tile that is copied next, and the holes of that tile.
+  int w_tile = t_first;  // first tile of the lanes' window
+  const char *kb = nullptr, *vb = nullptr;
+  int g_key = 0;
+  unsigned next_holes = 0;
+  bool g_live = false, g_whole = false;
+  auto aim = [&](int t) {
+    if (t - w_tile == WINDOW) {
+      w_tile = t;
+      gr.take(p, u, gran_of(t), gran_of(t + WINDOW));
+    }
+    const int at = (t - w_tile) * NW + w;
+    kb = kp + lane64(gr.ko, at);
+    vb = vp + lane64(gr.vo, at);
+    g_key = t * BN + w * kGranule;
+    g_live = (gr.live >> at) & 1;
+    g_whole = g_live && g_key >= u.lo && g_key + kGranule <= end;
+    next_holes = ~(unsigned)(gr.live >> ((t - w_tile) * NW)) & ((1u << NW) - 1);
+  };
+  auto issue = [&](int t) {
+    const uint32_t dst = smem_at + (uint32_t)((t & 1) * STAGE_B + w * GRAN_B);
+    if (!g_live) {
+      kc.zero(dst, lane);
+      vc.zero(dst + TILE_B, lane);
+    } else if (g_whole) {
+      kc.whole(dst, kb, k_ss_b);
+      vc.whole(dst + TILE_B, vb, v_ss_b);
+    } else {
+      const int first = max(0, u.lo - g_key), last = min(kGranule, end - g_key) - 1;
+      kc.part(dst, kb, k_ss_b, first, last);
+      vc.part(dst + TILE_B, vb, v_ss_b, first, last);
+    }
+  };
+
+  const Seen see = seen_by_wave(x);
+  State<D> st;
+  st.init();
+  const float c = score_coeff<SOFTCAP, 0>(p.s);
+  if (t_first < t_end) {
+    gr.take(p, u, gran_of(t_first), gran_of(t_first + WINDOW));
+    aim(t_first);
+    issue(t_first);
+  }
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) {
+    if (!x.ok) qf[kk] = V8{};
+    if constexpr (OCC == 1) asm volatile("" : "+a"(qf[kk]));
+    else asm volatile("" : "+v"(qf[kk]));
+  }
+
+  // One tile. Full tiles issue the next tile's copies one by one among their QK^T steps, so that the issue overlaps the
+  // MFMAs instead of following the barrier as one burst.
+  constexpr int CPS = (2 * LOADS + D / 16 - 1) / (D / 16);  // copies per QK^T step
+  auto tile = [&](const int t, const unsigned holes, auto masked) {
+    constexpr bool MASKED = decltype(masked)::value;
+    const uint32_t sto = (uint32_t)((t & 1) * STAGE_B);
+    uint32_t kbase[Fragments<D>::NK], vbase[Fragments<D>::NV];
+#pragma unroll
+    for (int i = 0; i < Fragments<D>::NK; ++i) {
+      kbase[i] = sto + fr.k[i];
+      asm volatile("" : "+v"(kbase[i]));
+    }
+#pragma unroll
+    for (int i = 0; i < Fragments<D>::NV; ++i) {
+      vbase[i] = sto + fr.v[i];
+      asm volatile("" : "+v"(vbase[i]));
+    }
+    bool blk_live[NMB], blk_full[NMB];
+    unsigned blk_holes[NMB];
+#pragma unroll
+    for (int mb = 0; mb < NMB; ++mb) {
+      const int kb0 = t * BN + koff + mb * 32;
+      blk_holes[mb] = MASKED ? (holes >> ((koff + mb * 32) / kGranule)) & 3u : 0u;
+      blk_live[mb] = !MASKED || (kb0 <= see.hi_max && kb0 + 31 >= see.lo_min && blk_holes[mb] != 3);
+      blk_full[mb] = !MASKED || (kb0 >= see.lo_max && kb0 + 31 <= see.hi_min && blk_holes[mb] == 0);
+    }
+    f32x16 sacc[NMB];
+#pragma unroll
+    for (int mb = 0; mb < NMB; ++mb) sacc[mb] = f32x16{};
+    if constexpr (MASKED) {
+#pragma unroll
+      for (int mb = 0; mb < NMB; ++mb) {
+        if (!blk_live[mb]) continue;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          sacc[mb] = mfma32(lds_read<V8>(kbase[fr.ki(kk)] + fr.ko(mb, kk)), qf[kk], sacc[mb]);
       }
     } else {
-      qi = i;
-      b = pl.b;
-      tok = pl.s.t0 + i;
-      n = pl.s.n;
-      kv = pl.s.kv;
-    }
-  }
-  const int h = hk * p.G + qg;
-  const int64_t q_off = p.cu_q != nullptr ? tok * p.q_ss : b * p.q_sb + qi * p.q_ss;
-
-  // Q fragment (B operand of S^T = K.Q^T): the row's head-dim elements 16kk + 8g .. +8.
-  const S* qp = static_cast<const S*>(p.q) + (row_ok ? q_off + h * p.q_sh : 0);
-  V8 qf[NKK];
+      const uint32_t dst = smem_at + (uint32_t)(((t + 1) & 1) * STAGE_B + w * GRAN_B);
 #pragma unroll
-  for (int kk = 0; kk < NKK; ++kk) qf[kk] = ld16<V8>(qp + 16 * kk + 8 * g);
+      for (int kk = 0; kk < D / 16; ++kk) {
 #pragma unroll
-  for (int kk = 0; kk < NKK; ++kk) {
-    asm volatile("" : "+v"(qf[kk]));
-    if (!row_ok) qf[kk] = V8{};
-  }
-
-  // Keys the row sees: k_lo <= key <= k_hi.
-  int k_hi = min(hi, kv) - 1, k_lo = lo;
-  if (p.causal) k_hi = min(k_hi, qi + kv - n);
-  if (p.window > 0) k_lo = max(k_lo, qi + kv - n - p.window + 1);
-  if (!row_ok) k_hi = k_lo - 1;
-  // Wave-uniform tile classes: a tile inside [lo_max, hi_min] is seen whole by every row of the wave (a row with no key
-  // in the unit makes every tile masked; lanes past the last row, whose results are dropped, do not count); a tile
-  // outside [lo_min, hi_max] is seen by none.
-  const bool empty = k_hi < k_lo;
-  const int lo_max = wave_max_i(!row_ok ? INT_MIN : empty ? INT_MAX : k_lo);
-  const int hi_min = wave_min_i(!row_ok ? INT_MAX : empty ? INT_MIN : k_hi);
-  const int lo_min = wave_min_i(row_ok && !empty ? k_lo : INT_MAX);
-  const int hi_max = wave_max_i(row_ok && !empty ? k_hi : INT_MIN);
-
-  // Page numbers: lane l holds those of granule gbase + l (64 granules are 32 tiles), as element offsets of the granule's
-  // first K and V row (negative: no such page); the next 64 are requested when these begin to be used.
-  const int32_t* trow = p.table + b_table * p.table_sb;
-  const int g_last = max(0, p.cap / kGranule - 1);
-  auto page_of = [&](int gi) { return trow[min(gi, g_last) / p.gpp]; };
-  auto offsets = [&](int gi, int page, int64_t& ko, int64_t& vo) {
-    const int in = (min(gi, g_last) % p.gpp) * kGranule;
-    const bool ok = page >= 0 && page < p.num_pages;
-    ko = ok ? page * p.k_sp + in * p.k_ss : -1;
-    vo = ok ? page * p.v_sp + in * p.v_ss : -1;
-  };
-  int gbase = 2 * t_begin;
-  int64_t ko_l = -1, vo_l = -1;
-  int page_next = 0;
-  if (t_begin < t_end) {
-    offsets(gbase + lane, page_of(gbase + lane), ko_l, vo_l);
-    page_next = page_of(gbase + 64 + lane);
-  }
-  auto lane64 = [&](int64_t x, int at) {
-    const unsigned lo32 = __builtin_amdgcn_readlane((int)(x & 0xffffffff), at);
-    const int hi32 = __builtin_amdgcn_readlane((int)(x >> 32), at);
-    return (int64_t)hi32 << 32 | lo32;
-  };
-
-  // Load i of a tile: thread tid reads 16-byte chunk tid % LPR of tile row i * RPI + tid / LPR, so one wave instruction
-  // covers 64 / LPR whole rows. A K / V row is read once by a decode unit: the loads are non-temporal.
-  const int krow = tid / LPR, c0 = tid % LPR;
-  const S* kp = static_cast<const S*>(p.k) + hk * p.k_sh + c0 * 8;
-  const S* vp = static_cast<const S*>(p.v) + hk * p.v_sh + c0 * 8;
-  V8 kreg[CPT], vreg[CPT];
-  int holes = 0;  // of the tile in the registers: bit 0 / 1, its first / second granule is no page; 3: nothing to see
-  auto load = [&](int t) {
-    if (2 * t - gbase >= 64) {
-      gbase += 64;
-      offsets(gbase + lane, page_next, ko_l, vo_l);
-      page_next = page_of(gbase + 64 + lane);
-    }
-    const int at = 2 * t - gbase, kt = t * BN;
-    const int64_t k0 = lane64(ko_l, at), k1 = lane64(ko_l, at + 1);
-    const int64_t v0 = lane64(vo_l, at), v1 = lane64(vo_l, at + 1);
-    holes = (k0 < 0 ? 1 : 0) | (k1 < 0 ? 2 : 0);
-    const int a = max(kt, lo) - kt, z = min(kt + BN, hi) - 1 - kt;  // rows of the tile that are keys of the unit
-    if (holes == 0 && a == 0 && z == BN - 1) {
+        for (int i = kk * CPS; i < std::min((kk + 1) * CPS, 2 * LOADS); ++i) {
+          if (i < LOADS) kc.one(dst, kb, k_ss_b, i);
+          else vc.one(dst + TILE_B, vb, v_ss_b, i - LOADS);
+        }
 #pragma unroll
-      for (int i = 0; i < CPT; ++i) {
-        const int rr = i * RPI + krow, in = rr & (kGranule - 1);
-        const bool second = rr >= kGranule;
-        kreg[i] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(kp + (second ? k1 : k0) + in * p.k_ss));
-        vreg[i] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(vp + (second ? v1 : v0) + in * p.v_ss));
+        for (int mb = 0; mb < NMB; ++mb)
+          sacc[mb] = mfma32(lds_read<V8>(kbase[fr.ki(kk)] + fr.ko(mb, kk)), qf[kk], sacc[mb]);
       }
-      return;
     }
-    // An edge tile, or one with a hole: rows that are no key read one that is.
-    if (z < kGranule) holes |= 2;
-    if (a >= kGranule) holes |= 1;
-    if (holes == 3) return;
-    const int spare = (holes & 1) ? max(a, kGranule) : a;
-#pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-      int rr = i * RPI + krow;
-      const bool ok = rr >= a && rr <= z && !(holes & (rr >= kGranule ? 2 : 1));
-      rr = ok ? rr : spare;
-      const int in = rr & (kGranule - 1);
-      const bool second = rr >= kGranule;
-      kreg[i] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(kp + (second ? k1 : k0) + in * p.k_ss));
-      vreg[i] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(vp + (second ? v1 : v0) + in * p.v_ss));
-    }
-  };
-  auto store = [&]() {
-#pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-      *reinterpret_cast<V8*>(&Ks[i * RPI + krow][c0 * 8]) = kreg[i];
-      *reinterpret_cast<V8*>(&Vs[i * RPI + krow][c0 * 8]) = vreg[i];
-    }
-  };
-
-  f32x16 oacc[NDB];
-#pragma unroll
-  for (int i = 0; i < NDB; ++i) oacc[i] = f32x16{};
-  float m_run = -INFINITY;  // reference maximum (value units)
-  float l_part[4] = {0.f, 0.f, 0.f, 0.f};
-  const float c = score_coeff<SOFTCAP, 0>(p.s);
-  const int tr_krow = (lane & 15) >> 2;                         // key row within a group of 4
-  const int tr_dcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);  // head-dim column within a 32-wide block
-
-  auto tile = [&](const int kt, const int hole, auto masked) {
-    f32x16 sacc = f32x16{};
-#pragma unroll
-    for (int kk = 0; kk < NKK; ++kk) {
-      const V8 a = *reinterpret_cast<const V8*>(&Ks[r][16 * kk + 8 * g]);
-      sacc = mfma32(a, qf[kk], sacc);
-    }
-    // element j holds key kt + 8*(j/4) + 4g + j%4
-    const int rel_hi = k_hi - (kt + 4 * g), rel_lo = k_lo - (kt + 4 * g);
     float mloc = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      float x = score_value<T, SOFTCAP, 0>(sacc[j], p.s);
-      if constexpr (decltype(masked)::value) {
-        const int o = 8 * (j >> 2) + (j & 3);
-        x = (o <= rel_hi && o >= rel_lo && !(hole & (j < 8 ? 1 : 2))) ? x : -INFINITY;
+    for (int mb = 0; mb < NMB; ++mb) {
+      const int k4 = t * BN + koff + mb * 32 + 4 * g;
+      if (MASKED && !blk_live[mb]) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sacc[mb][j] = -INFINITY;
+      } else if (MASKED && !blk_full[mb]) {
+        mloc = fmaxf(mloc, block_scores<T, SOFTCAP, true>(sacc[mb], p, x.k_lo - k4, x.k_hi - k4, blk_holes[mb]));
+      } else {
+        mloc = fmaxf(mloc, block_scores<T, SOFTCAP, false>(sacc[mb], p, 0, 0, 0));
       }
-      sacc[j] = x;
-      mloc = fmaxf(mloc, x);
     }
-    mloc = half_swap_max(mloc);
-    const float m_new = fmaxf(m_run, mloc);
-    const bool need = m_new * c > m_run * c + kRescaleThreshold;
-    if (__any(need)) {
-      const float alpha = need ? fast_exp2((m_run - m_new) * c) : 1.0f;
-      if (need) m_run = m_new;
+    st.raise(mloc, c);
+    const float mc = st.m == -INFINITY ? 0.f : st.m * c;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) l_part[i] *= alpha;
-#pragma unroll
-      for (int i = 0; i < NDB; ++i) oacc[i] *= alpha;
-    }
-    const float mc = m_run == -INFINITY ? 0.f : m_run * c;
-#pragma unroll
-    for (int kk = 0; kk < NPK; ++kk) {
+    for (int kk = 0; kk < SBN / 16; ++kk) {
+      if (MASKED && !blk_live[kk >> 1]) continue;  // P = 0 there
       f32x8 pv;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float pe = fast_exp2(fmaf(sacc[8 * kk + e], c, -mc));
-        l_part[e & 3] += pe;
+        const float pe = fast_exp2(fmaf(sacc[kk >> 1][8 * (kk & 1) + e], c, -mc));
+        st.l[e & 1] += pe;
         pv[e] = pe;
       }
       const V8 pb = from_f32x8<V8>(pv);
 #pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        // A = V^T rows db*32 + r, keys 16kk + 4g + {0..3} and 16kk + 8 + 4g + {0..3} (the P operand's key order)
-        const S* vrow = &Vs[16 * kk + 4 * g + tr_krow][db * 32 + tr_dcol];
-        const V4 lo4 = tr_read(vrow);
-        const V4 hi4 = tr_read(vrow + 8 * KP);
-        oacc[db] = mfma32(__builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7), pb, oacc[db]);
+      for (int db = 0; db < D / 32; ++db) {
+        const V4 a0 = tr_read_at(vbase[fr.vb(db, 0)] + fr.vo(kk, 0), S{});
+        const V4 a1 = tr_read_at(vbase[fr.vb(db, 1)] + fr.vo(kk, 1), S{});
+        st.o[db] = mfma32(__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7), pb, st.o[db]);
       }
     }
   };
 
-  if (t_begin < t_end) load(t_begin);
-  for (int t = t_begin; t < t_end; ++t) {
-    const int hole = holes;
-    if (hole != 3) store();
+  for (int t = t_first; t < t_end; ++t) {
+    wait_vmem<0>();
     __syncthreads();
-    if (t + 1 < t_end) load(t + 1);  // in flight during this tile's compute
-    const int kt = t * BN;
-    if (hole != 3 && kt <= hi_max && kt + BN - 1 >= lo_min) {
-      if (hole == 0 && kt >= lo_max && kt + BN - 1 <= hi_min) tile(kt, 0, std::false_type{});
-      else tile(kt, hole, std::true_type{});
+    const unsigned holes = next_holes;
+    const int kb0 = t * BN + koff;
+    const bool more = t + 1 < t_end;
+    if (more) aim(t + 1);
+    const bool full = holes == 0 && kb0 >= see.lo_max && kb0 + SBN - 1 <= see.hi_min;
+    if (full && more && g_whole) {
+      tile(t, 0, std::false_type{});
+    } else {
+      if (more) issue(t + 1);
+      if (kb0 <= see.hi_max && kb0 + SBN - 1 >= see.lo_min) tile(t, holes, std::true_type{});
     }
-    __syncthreads();
   }
 
-  const float l_tot = half_swap_sum((l_part[0] + l_part[1]) + (l_part[2] + l_part[3]));
-  if (!row_ok) return;
-  if (slot < 0) {
-    const float inv = l_tot == 0.f ? 0.f : 1.0f / l_tot;  // a row that sees no key: o = 0, lse = -inf
-    S* op = static_cast<S*>(p.o) + (p.cu_q != nullptr ? tok * p.o_ss : b * p.o_sb + qi * p.o_ss) + h * p.o_sh;
-#pragma unroll
-    for (int db = 0; db < NDB; ++db)
-#pragma unroll
-      for (int jj = 0; jj < 4; ++jj) {
-        V4 ov;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) ov[e] = to_s<S>(oacc[db][4 * jj + e] * inv);
-        *reinterpret_cast<V4*>(op + db * 32 + 8 * jj + 4 * g) = ov;
-      }
-    if (p.lse != nullptr && g == 0)
-      p.lse[(int64_t)tok * p.Hq + h] = l_tot == 0.f ? -INFINITY : (m_run * c + fast_log2(l_tot)) * kLn2;
-    return;
-  }
-  if (slot >= p.slots) return;  // (only where cu_q descends)
-  // Partial of this unit for the lane's row: unnormalised O, maximum (exp2 domain), sum.
-  const int64_t pidx = ((int64_t)slot * p.Hkv + hk) * p.rows_stride + rl;
-  float* po = p.part_o + pidx * D;
-#pragma unroll
-  for (int db = 0; db < NDB; ++db)
-#pragma unroll
-    for (int jj = 0; jj < 4; ++jj)
-      *reinterpret_cast<f32x4*>(po + db * 32 + 8 * jj + 4 * g) =
-          f32x4{oacc[db][4 * jj], oacc[db][4 * jj + 1], oacc[db][4 * jj + 2], oacc[db][4 * jj + 3]};
-  if (g == 0) {
-    p.part_ml[pidx * 2 + 0] = m_run == -INFINITY ? -INFINITY : m_run * c;
-    p.part_ml[pidx * 2 + 1] = l_tot;
+  // States go through the LDS, so that the stores cover whole rows; KG states of a row are joined.
+  f32x2* ml = reinterpret_cast<f32x2*>(smem + NW * SLOT_B);
+  __syncthreads();  // every wave is done with the tiles
+  put_state(st, smem + w * SLOT_B, ml + 32 * w, c, lane);
+  __syncthreads();
+  const int live_rows = min(32 * NWR, u.rows - u.row0);
+  for (int it = tid; it < live_rows * (D / 8); it += 64 * NW) {
+    const int row = it / (D / 8), quad = it % (D / 8);
+    const Row y = find_row(p, u, row, hk);
+    if (!y.ok) continue;
+    write_row<T, D, KG>(p, u, smem + (row / 32) * SLOT_B, ml + 32 * (row / 32), NWR, SLOT_B, row % 32, quad, y.o,
+                        (int64_t)y.tok * p.Hq + y.h, row, hk);
   }
 }
 
-// Joins the partials of a row: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, lse = (M + log2 L) ln 2, with the
-// prefix slices first and then the sequence's own. One wave per row at a time: its lanes hold the head dim.
+// Joins the partials of rows: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, lse = (M + log2 L) ln 2, with the prefix
+// slices first and then the sequence's own. ROWS rows at a time per workgroup of 256: 256 / ROWS threads to a row, in
+// groups of D / 4 (four head-dim elements each) that take the slices in turn.
 constexpr int kMergeThreads = 256;
-template <typename T, int D>
+template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(PagedParams p, int rows_per_wg) {
   typedef typename T::scalar S;
-  constexpr int E = D / 64;  // elements per lane
-  typedef float fE __attribute__((ext_vector_type(E)));
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  typedef typename T::vec4 V4;
+  constexpr int COLS = D / 4, NG = kMergeThreads / (COLS * ROWS);
+  static_assert(NG >= 1 && NG * COLS * ROWS == kMergeThreads, "threads");
+  __shared__ f32x4 part[ROWS][NG][COLS];
+  __shared__ f32x2 part_ml[ROWS][NG];
+  const int tid = threadIdx.x, lane = tid & 63;
   const int hk = blockIdx.y;
   const Division dv = divide(p, lane);
   const Place pl = find_place<false>(p, dv, blockIdx.x, lane);
   if (pl.b < 0 || (p.P == 0 && pl.ns == 1)) return;
   const int rows = min(pl.s.n * p.G - pl.local * p.R, p.R);
-  const int p_units = dv.p_rg * dv.p_ns;
-  const int slot0 = p_units + pl.slot + pl.local * pl.ns;
+  const int slot0 = dv.p_rg * dv.p_ns + pl.slot + pl.local * pl.ns;
   if (slot0 + pl.ns > p.slots) return;  // (only where cu_q descends)
-  for (int rl = blockIdx.z * rows_per_wg + wv; rl < min(rows, (int)(blockIdx.z + 1) * rows_per_wg);
-       rl += kMergeThreads / 64) {
-    const int row = pl.local * p.R + rl;
-    const int qi = row / p.G, tok = pl.s.t0 + qi, h = hk * p.G + (row - qi * p.G);
-    const int prow = tok * p.G + (row - qi * p.G);
-    const int prg = prow / p.R, prl = prow - prg * p.R;
-    const int n_all = dv.p_ns + pl.ns;
-    auto index = [&](int i) {
-      const int64_t s = i < dv.p_ns ? prg * dv.p_ns + i : slot0 + (i - dv.p_ns);
-      return (s * p.Hkv + hk) * p.rows_stride + (i < dv.p_ns ? prl : rl);
-    };
-    float M = -INFINITY;
-    for (int i = lane; i < n_all; i += 64) M = fmaxf(M, p.part_ml[index(i) * 2]);
-    M = wave_max(M);
-    const float Mu = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
-    fE acc = {};
-    for (int i = 0; i < n_all; ++i) {
-      const int64_t x = index(i);
-      const float wgt = fast_exp2(p.part_ml[x * 2] - Mu);
-      L = fmaf(wgt, p.part_ml[x * 2 + 1], L);
-      acc += wgt * *reinterpret_cast<const fE*>(p.part_o + x * D + lane * E);
-    }
-    const float inv = L == 0.f ? 0.f : 1.0f / L;
-    S* op = static_cast<S*>(p.o) + (p.cu_q != nullptr ? tok * p.o_ss : pl.b * p.o_sb + qi * p.o_ss) + h * p.o_sh + lane * E;
-    if constexpr (E == 1) {
-      op[0] = to_s<S>(acc[0] * inv);
-    } else {
-      typedef S sE __attribute__((ext_vector_type(E)));
-      sE ov;
+  const int col = tid % COLS, grp = tid / COLS % NG, rr = tid / (COLS * NG);
+  const int n_all = dv.p_ns + pl.ns;
+  const int64_t slot_rows = (int64_t)p.Hkv * p.rows_stride;
+  for (int r0 = blockIdx.z * rows_per_wg; r0 < min(rows, (int)(blockIdx.z + 1) * rows_per_wg); r0 += ROWS) {
+    const int rl = r0 + rr;
+    const bool ok = rl < rows;
+    const int row = pl.local * p.R + min(rl, rows - 1);
+    const int qi = row / p.G, qg = row - qi * p.G, tok = pl.s.t0 + qi, h = hk * p.G + qg;
+    const int prow = tok * p.G + qg, prg = prow / p.R, prl = prow - prg * p.R;
+    // partial i of this row: prefix slice i, or slice i - p_ns of the sequence
+    const int64_t own = ((int64_t)(slot0 - dv.p_ns) * p.Hkv + hk) * p.rows_stride + min(rl, rows - 1);
+    const int64_t pre = ((int64_t)prg * dv.p_ns * p.Hkv + hk) * p.rows_stride + prl;
+    float M = -INFINITY, Ls = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    constexpr int U = 4;  // partials in flight
+    for (int i0 = grp; i0 < n_all; i0 += NG * U) {
+      f32x4 o[U];
+      f32x2 x[U];
 #pragma unroll
-      for (int e = 0; e < E; ++e) ov[e] = to_s<S>(acc[e] * inv);
-      *reinterpret_cast<sE*>(op) = ov;
+      for (int k = 0; k < U; ++k) {
+        const int i = min(i0 + NG * k, n_all - 1);
+        const int64_t at = (i < dv.p_ns ? pre : own) + i * slot_rows;
+        x[k] = *reinterpret_cast<const f32x2*>(p.part_ml + 2 * at);
+        o[k] = *reinterpret_cast<const f32x4*>(p.part_o + at * D + 4 * col);
+      }
+      float m = M;
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        if (i0 + NG * k >= n_all) x[k] = f32x2{-INFINITY, 0.f};
+        m = fmaxf(m, x[k][0]);
+      }
+      const float mu = m == -INFINITY ? 0.f : m, a = fast_exp2(M - mu);
+      acc *= a;
+      Ls *= a;
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const float wgt = fast_exp2(x[k][0] - mu);
+        acc += wgt * o[k];
+        Ls = fmaf(wgt, x[k][1], Ls);
+      }
+      M = m;
     }
-    if (p.lse != nullptr && lane == 0)
-      p.lse[(int64_t)tok * p.Hq + h] = L == 0.f ? -INFINITY : (M + fast_log2(L)) * kLn2;
+    if constexpr (NG > 1) {
+      part[rr][grp][col] = acc;
+      if (col == 0) part_ml[rr][grp] = f32x2{M, Ls};
+      __syncthreads();
+      if (grp == 0) {
+        M = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) M = fmaxf(M, part_ml[rr][i][0]);
+        const float mu = M == -INFINITY ? 0.f : M;
+        Ls = 0.f;
+        acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          const float wgt = fast_exp2(part_ml[rr][i][0] - mu);
+          Ls = fmaf(wgt, part_ml[rr][i][1], Ls);
+          acc += wgt * part[rr][i][col];
+        }
+      }
+      __syncthreads();
+      if (grp != 0) continue;
+    }
+    if (!ok) continue;
+    const float inv = Ls == 0.f ? 0.f : 1.0f / Ls;
+    S* op = static_cast<S*>(p.o) + (p.cu_q != nullptr ? tok * p.o_ss : pl.b * p.o_sb + qi * p.o_ss) + h * p.o_sh;
+    V4 ov;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ov[e] = to_s<S>(acc[e] * inv);
+    *reinterpret_cast<V4*>(op + 4 * col) = ov;
+    if (p.lse != nullptr && col == 0)
+      p.lse[(int64_t)tok * p.Hq + h] = Ls == 0.f ? -INFINITY : (M + fast_log2(Ls)) * kLn2;
   }
 }
 
 // The host's part of the division.
 struct HostPlan {
-  int nw, R, rows_stride, target, min_slice, grid_units, slots, merge_units;
+  int R, rows_stride, target, min_slice, grid_units, slots, merge_units;
 };
 HostPlan host_plan(int64_t B, int64_t T, bool ragged, int64_t Hq, int64_t Hkv, int64_t D, int64_t P) {
   HostPlan h{};
   const int64_t G = Hq / Hkv, Sq = B > 0 ? T / B : 0;
-  const int64_t most = (ragged ? T : Sq) * G;             // most rows that a sequence can have
-  const int64_t mean = B > 0 ? (T * G + B - 1) / B : 0;   // rows of the average one
-  const int64_t typical = ragged ? std::max<int64_t>(mean, 1) : most;
-  h.nw = std::max<int64_t>(typical, P > 0 ? std::min<int64_t>(T * G, 64) : 0) <= 32 ? 1 : typical <= 64 ? 2 : 4;
-  if (P > 0 && T * G > 64) h.nw = 4;
-  if (D == 256 && h.nw == 1) h.nw = 2;
-  h.R = 32 * h.nw;
+  const int64_t most = (ragged ? T : Sq) * G;  // most rows that a sequence can have
+  // Rows that a workgroup finds to do: those of the average sequence (of the batch, where there is a prefix).
+  const int64_t typical = P > 0 ? T * G : ragged ? (T * G + B - 1) / B : most;
+  const int widest = D == 128 ? 256 : 128;
+  h.R = typical <= 32 ? 32 : typical <= 64 ? 64 : typical <= 128 || widest == 128 ? 128 : 256;
   h.rows_stride = (int)std::min<int64_t>(h.R, P > 0 ? T * G : most);
-  h.target = (int)std::max<int64_t>(1024, Hkv);
-  h.min_slice = 2;
+  h.target = (int)std::max<int64_t>(h.R == 32 ? 2048 : 768, Hkv);
+  h.min_slice = h.R == 32 ? 1 : 2;
   const int64_t nrg = ragged ? T * G / h.R + std::min(B, T) : B * ((Sq * G + h.R - 1) / h.R);
   const int64_t p_rg = P > 0 ? (T * G + h.R - 1) / h.R : 0;
   h.merge_units = (int)nrg;
@@ -408,22 +821,34 @@ HostPlan host_plan(int64_t B, int64_t T, bool ragged, int64_t Hq, int64_t Hkv, i
   return h;
 }
 
-template <typename T, int D, int NW>
-void launch_nw(const PagedParams& p, const HostPlan& h, hipStream_t st) {
+template <typename T, int D, bool SOFTCAP>
+void launch_cap(const PagedParams& p, const HostPlan& h, hipStream_t st) {
   const dim3 grid(h.grid_units, p.Hkv);
-  if (p.s.softcap > 0.f)
-    hipLaunchKernelGGL((paged_attn_kernel<T, D, NW, true>), grid, dim3(64 * NW), 0, st, p);
-  else
-    hipLaunchKernelGGL((paged_attn_kernel<T, D, NW, false>), grid, dim3(64 * NW), 0, st, p);
-  const int rpw = h.rows_stride <= 32 ? 4 : 32;
-  hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3(h.merge_units, p.Hkv, (h.rows_stride + rpw - 1) / rpw),
-                     dim3(kMergeThreads), 0, st, p, rpw);
+  if (h.R == 32)
+    hipLaunchKernelGGL((paged_narrow_kernel<T, D, SOFTCAP>), grid, dim3(64 * kNarrowWaves), 0, st, p);
+  else if constexpr (D == 128) {
+    if (h.R == 64) hipLaunchKernelGGL((paged_wide_kernel<T, D, 8, 4, 2, SOFTCAP>), grid, dim3(512), 0, st, p);
+    else if (h.R == 128) hipLaunchKernelGGL((paged_wide_kernel<T, D, 8, 2, 2, SOFTCAP>), grid, dim3(512), 0, st, p);
+    else hipLaunchKernelGGL((paged_wide_kernel<T, D, 8, 1, 2, SOFTCAP>), grid, dim3(512), 0, st, p);
+  } else {
+    constexpr int OCC = D == 64 ? 3 : 1;
+    if (h.R == 64) hipLaunchKernelGGL((paged_wide_kernel<T, D, 4, 2, OCC, SOFTCAP>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((paged_wide_kernel<T, D, 4, 1, OCC, SOFTCAP>), grid, dim3(256), 0, st, p);
+  }
 }
 template <typename T, int D>
 void launch(const PagedParams& p, const HostPlan& h, hipStream_t st) {
-  if (h.nw == 4) return launch_nw<T, D, 4>(p, h, st);
-  if (h.nw == 2) return launch_nw<T, D, 2>(p, h, st);
-  if constexpr (D < 256) launch_nw<T, D, 1>(p, h, st);
+  if (p.s.softcap > 0.f) launch_cap<T, D, true>(p, h, st);
+  else launch_cap<T, D, false>(p, h, st);
+  if (h.rows_stride <= 32) {
+    hipLaunchKernelGGL((paged_merge_kernel<T, D, 1>), dim3(h.merge_units, p.Hkv, h.rows_stride), dim3(kMergeThreads), 0,
+                       st, p, 1);
+  } else {
+    constexpr int ROWS = kMergeThreads / (D / 4);
+    const int rpw = 32;
+    hipLaunchKernelGGL((paged_merge_kernel<T, D, ROWS>), dim3(h.merge_units, p.Hkv, (h.rows_stride + rpw - 1) / rpw),
+                       dim3(kMergeThreads), 0, st, p, rpw);
+  }
 }
 
 int check_sizes(const char* op, int64_t B, int64_t T, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix) {
@@ -480,6 +905,9 @@ extern "C" int dgg_attn_paged(const void* q, const void* k_pages, const void* v_
   for (int i = 0; i < 12; ++i)
     DGG_REQUIRE(strides[i] >= 0 && strides[i] % 8 == 0, DGG_ERR_STRIDE,
                 "%s: stride[%d] = %lld must be a non-negative multiple of 8 elements", op, i, (long long)strides[i]);
+  DGG_REQUIRE(strides[4] < (1 << 24) && strides[7] < (1 << 24), DGG_ERR_STRIDE,
+              "%s: a page's rows are too far apart (strides %lld, %lld; fewer than 2^24 elements)", op,
+              (long long)strides[4], (long long)strides[7]);
   DGG_REQUIRE(strides[12] >= 0, DGG_ERR_STRIDE, "%s: the block table's row stride is negative", op);
   if (B == 0 || T == 0) return DGG_OK;
   DGG_REQUIRE(q && o && kv_lens, DGG_ERR_NULL, "%s: null q/o/kv_lens pointer", op);
@@ -525,8 +953,8 @@ extern "C" int dgg_attn_paged(const void* q, const void* k_pages, const void* v_
   p.window = (int)std::min<int64_t>(window, 1 << 30);
   p.R = h.R;
   p.rows_stride = h.rows_stride;
-  p.target = h.target;
   p.min_slice = h.min_slice;
+  p.per_target = (float)((1.0 + 1.0 / 2048) * (double)Hkv / (double)h.target);
   p.grid_units = h.grid_units;
   p.slots = h.slots;
   hipStream_t st = dgg::as_stream(stream);
