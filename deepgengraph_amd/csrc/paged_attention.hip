@@ -7,16 +7,17 @@
 //   S^T (32 keys x 32 rows) = K . Q^T     v_mfma_f32_32x32x16, A = K from the LDS, B = Q in registers
 //   O^T (D x 32 rows)      += V^T . P^T   A = V^T by transposing LDS reads, B = P from the S^T accumulator
 // with one running maximum and sum per row, in fp32; P is rounded to the storage type, as the matrix instruction takes it
-// (its error is that of the output's own rounding, spread over the keys). Two kernels:
-//   narrow  up to 32 rows of a KV head: bound by the stream of keys and values. Four waves share the rows and take the
+// (its error is that of the output's own rounding, spread over the keys). Two ways:
+//   narrow  up to 32 rows of a KV head: bound by the stream of keys and values. The waves share the rows and take the
 //           32-key tiles in turn, each with buffers of its own and no barrier, and add their states at the end;
 //   wide    more rows: bound by the matrix products. The waves share the tiles and have rows of their own.
-// Partials of split rows are joined by a third.
+// Batches that may hold both run in one launch of workgroups that can do either. Partials are joined by the merge.
 //
 // A granule is 16 keys, which lie in one page one after another. Granules that hold no key of the unit (behind kv_len,
 // before the window, on a page number outside the pool) are zeros in the LDS and masked; rows of a granule that are no
 // keys are replaced by one that is. What memory holds there does not matter.
 #include <climits>
+#include <cstdlib>
 
 #include "common.h"
 
@@ -28,54 +29,33 @@ namespace {
 using namespace dgg_attn;
 using namespace dgg_paged;
 
-// The unit of this workgroup and its keys.
+// A unit of work: rows and keys.
 struct Unit {
   bool prefix;
   int b;          // sequence (prefix: 0, whose table it reads)
   Seq s;
   int row0, rows; // first row; rows of the row space (the sequence's, or the whole batch's)
-  int slot;       // partial slot, or -1: the unit writes the output
   int lo, hi;     // keys of it that any row of the row group sees
-  int k0, k1;     // keys of the slice (k0 a multiple of kTile); those of [lo, hi) count
+  int k0, k1;     // keys of the unit (k0 a multiple of kTile); those of [lo, hi) count
+  bool whole;     // the unit writes the output; otherwise a partial, to:
+  float* part_o;  // row 0 of its slot
+  float* part_ml;
 };
-__device__ __forceinline__ bool find_unit(const PagedParams& p, int lane, Unit& u) {
-  const Division dv = divide(p, lane);
-  const int p_units = dv.p_rg * dv.p_ns;
-  const int bid = blockIdx.x;
-  u.prefix = bid < p_units;
-  int k, ns;
-  if (u.prefix) {
-    k = bid / dv.p_rg;
-    const int rg = bid - k * dv.p_rg;
-    ns = dv.p_ns;
-    u.b = 0;
-    u.row0 = rg * p.R;
-    u.rows = p.T * p.G;
-    u.slot = rg * dv.p_ns + k;
-    u.lo = dv.p_lo;
-    u.hi = p.P;
-  } else {
-    const Place pl = find_place<true>(p, dv, bid - p_units, lane);
-    if (pl.b < 0) return false;
-    const int nrg = row_groups(p, pl.s);
-    k = pl.local / nrg;
-    const int rg = pl.local - k * nrg;
-    ns = pl.ns;
-    u.b = pl.b;
-    u.s = pl.s;
-    u.row0 = rg * p.R;
-    u.rows = pl.s.n * p.G;
-    u.slot = p.P > 0 || pl.ns > 1 ? p_units + pl.slot + rg * pl.ns + k : -1;
-    const int off = pl.s.kv - pl.s.n;
-    u.lo = first_key(p, pl.s);
-    u.hi = pl.s.kv;
-    if (p.causal) u.hi = min(u.hi, (min(u.row0 + p.R, u.rows) - 1) / p.G + off + 1);
-    if (p.window > 0) u.lo = max(u.lo, u.row0 / p.G + off - p.window + 1);
-  }
-  const int tiles = key_tiles(u.lo, u.hi), per = ceil_div(tiles, ns), t0 = u.lo / kTile;
-  u.k0 = (t0 + min(tiles, k * per)) * kTile;
-  u.k1 = (t0 + min(tiles, (k + 1) * per)) * kTile;
-  return true;
+template <int D>
+__device__ __forceinline__ void use_slot(const PagedParams& p, Unit& u, bool wide, int slot, int hk) {
+  const int64_t row = ((int64_t)slot * p.Hkv + hk) * (wide ? p.wide_rows : p.narrow_rows);
+  // (a slot past the last: only where cu_q descends)
+  const bool ok = slot < (wide ? p.wide_slots : p.narrow_slots);
+  u.part_ml = ok ? (wide ? p.wide_ml : p.narrow_ml) + row * 2 : nullptr;
+  u.part_o = (wide ? p.wide_o : p.narrow_o) + row * D;
+}
+// Keys that the rows row0 .. of the sequence see.
+__device__ __forceinline__ void set_range(const PagedParams& p, Unit& u, int most_rows) {
+  const int off = u.s.kv - u.s.n;
+  u.lo = first_key(p, u.s);
+  u.hi = u.s.kv;
+  if (p.causal) u.hi = min(u.hi, (min(u.row0 + most_rows, u.rows) - 1) / p.G + off + 1);
+  if (p.window > 0) u.lo = max(u.lo, u.row0 / p.G + off - p.window + 1);
 }
 
 // A query row of the unit, as a lane holds it.
@@ -88,7 +68,7 @@ struct Row {
 __device__ __forceinline__ Row find_row(const PagedParams& p, const Unit& u, int rl, int hk) {
   Row x{};
   const int row = u.row0 + rl;
-  x.ok = row < u.rows && rl < p.R;
+  x.ok = row < u.rows;
   int i = 0, b = u.b;
   Seq s = u.s;
   if (x.ok) {
@@ -160,9 +140,19 @@ __device__ __forceinline__ int64_t lane64(int64_t x, int at) {
   return (int64_t)hi32 << 32 | lo32;
 }
 
+// dma16 (attention_common.h), with the non-temporal hint for NT: rows that one workgroup reads once.
+template <bool NT>
+__device__ __forceinline__ void copy16(uint32_t lds, const void* sbase, uint32_t voff) {
+  if constexpr (NT)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(voff), "s"(sbase)
+                 : "memory", "m0");
+  else
+    dma16(lds, sbase, voff);
+}
+
 // Copies one granule (16 rows of D) of K or V to `lds`, the place of its first 4- or 8-row group. kWhole: every row is a
 // key. Otherwise rows outside [first, last] are replaced by the nearest that is inside.
-template <int D>
+template <int D, bool NT>
 struct GranuleCopy {
   typedef DmaLayout<D> L;
   static constexpr int LOADS = kGranule / L::RPI;  // direct loads per granule
@@ -185,7 +175,7 @@ struct GranuleCopy {
     return (uint32_t)((i / L::IPG) * L::GROUP_B + (i % L::IPG) * L::RPI * L::ROW_B);
   }
   __device__ __forceinline__ void one(uint32_t lds, const char* base, int64_t ss_b, int i) const {
-    dma16(lds + place(i), base + (int64_t)(D == 64 ? i * L::RPI : (i / L::IPG) * L::GR) * ss_b, voff[vi(i)]);
+    copy16<NT>(lds + place(i), base + (int64_t)(D == 64 ? i * L::RPI : (i / L::IPG) * L::GR) * ss_b, voff[vi(i)]);
   }
   __device__ __forceinline__ void whole(uint32_t lds, const char* base, int64_t ss_b) const {
 #pragma unroll
@@ -302,18 +292,17 @@ __device__ __forceinline__ void write_row(const PagedParams& p, const Unit& u, c
     lo += wt[i] * *reinterpret_cast<const f32x4*>(s);
     hi += wt[i] * *reinterpret_cast<const f32x4*>(s + 32 * 16);
   }
-  if (u.slot < 0) {
+  if (u.whole) {
     const float inv = l == 0.f ? 0.f : 1.0f / l;  // a row that sees no key: o = 0, lse = -inf
     st16(static_cast<S*>(p.o) + o_off + 8 * quad,
          from_f32x8<V8>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7) * inv));
     if (p.lse != nullptr && quad == 0) p.lse[tok_h] = l == 0.f ? -INFINITY : (m + fast_log2(l)) * kLn2;
     return;
   }
-  if (u.slot >= p.slots) return;  // (only where cu_q descends)
-  const int64_t x = ((int64_t)u.slot * p.Hkv + hk) * p.rows_stride + rl;
-  *reinterpret_cast<f32x4*>(p.part_o + x * D + 8 * quad) = lo;
-  *reinterpret_cast<f32x4*>(p.part_o + x * D + 8 * quad + 4) = hi;
-  if (quad == 0) *reinterpret_cast<f32x2*>(p.part_ml + 2 * x) = f32x2{m, l};
+  if (u.part_ml == nullptr) return;
+  *reinterpret_cast<f32x4*>(u.part_o + (int64_t)rl * D + 8 * quad) = lo;
+  *reinterpret_cast<f32x4*>(u.part_o + (int64_t)rl * D + 8 * quad + 4) = hi;
+  if (quad == 0) *reinterpret_cast<f32x2*>(u.part_ml + 2 * rl) = f32x2{m, l};
 }
 
 // Scores of one 32-key block in the exp2 domain's value units, masked where `masked`; returns their maximum.
@@ -333,28 +322,30 @@ __device__ __forceinline__ float block_scores(f32x16& s, const PagedParams& p, i
   return mloc;
 }
 
-constexpr int kNarrowWaves = 4;
+// LDS of the two ways: NW waves' K and V buffers (which their O takes afterwards) and row states; two stages of a tile of
+// 16 keys per wave.
+template <int D, int NW>
+struct Lds {
+  typedef DmaLayout<D> L;
+  static constexpr int TILE_B = (32 / L::GR) * L::GROUP_B;  // K or V rows of 32 keys
+  static constexpr int GRAN_B = (kGranule / L::GR) * L::GROUP_B;
+  static constexpr int SLOT_B = (D / 8) * kOQ;
+  static constexpr int WAVE_B = std::max(2 * TILE_B, SLOT_B);
+  static constexpr int NARROW = NW * (WAVE_B + 32 * 8);
+  static constexpr int WIDE = std::max(2 * 2 * NW * GRAN_B, NW * (SLOT_B + 32 * 8));
+};
 
-// Waves per SIMD: as many workgroups per CU as the LDS holds (33 KiB at head_dim 64, 67 at 128, 133 at 256).
-template <typename T, int D, bool SOFTCAP>
-__global__ void __launch_bounds__(64 * kNarrowWaves)
-__attribute__((amdgpu_waves_per_eu(D >= 256 ? 1 : D >= 128 ? 2 : 4))) paged_narrow_kernel(PagedParams p) {
+// One narrow unit: its keys over NW waves.
+template <typename T, int D, int NW, bool SOFTCAP>
+__device__ __forceinline__ void narrow_unit(const PagedParams& p, const Unit& u, char* smem, int hk) {
   typedef DmaLayout<D> L;
   typedef typename T::scalar S;
   typedef typename T::vec8 V8;
   typedef typename T::vec4 V4;
-  constexpr int NW = kNarrowWaves;
-  constexpr int TILE_B = (32 / L::GR) * L::GROUP_B;  // K or V rows of 32 keys
-  constexpr int GRAN_B = (kGranule / L::GR) * L::GROUP_B;
-  constexpr int LOADS = 2 * GranuleCopy<D>::LOADS;   // direct loads of a tile, K or V
-  constexpr int WAVE_B = std::max(2 * TILE_B, (D / 8) * kOQ);
-  __shared__ __attribute__((aligned(1024))) char smem[NW * (WAVE_B + 32 * 8)];
-
+  constexpr int TILE_B = Lds<D, NW>::TILE_B, GRAN_B = Lds<D, NW>::GRAN_B, WAVE_B = Lds<D, NW>::WAVE_B;
+  constexpr int LOADS = 2 * GranuleCopy<D, true>::LOADS;   // direct loads of a tile, K or V
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hk = blockIdx.y;
-  Unit u;
-  if (!find_unit(p, lane, u)) return;
 
   // The wave's tiles: every NW-th of the slice's 32-key tiles that hold a key.
   const int t_first = max(u.k0, u.lo) / 32, t_end = ceil_div(min(u.k1, u.hi), 32);
@@ -373,7 +364,7 @@ __attribute__((amdgpu_waves_per_eu(D >= 256 ? 1 : D >= 128 ? 2 : 4))) paged_narr
 
   const uint32_t wave_at = (uint32_t)(size_t)((lds_char*)smem) + w * WAVE_B;
   const int64_t k_ss_b = 2 * p.k_ss, v_ss_b = 2 * p.v_ss;
-  GranuleCopy<D> kc, vc;
+  GranuleCopy<D, true> kc, vc;
   kc.init(lane, k_ss_b);
   vc.init(lane, v_ss_b);
   Fragments<D> fr;
@@ -390,7 +381,7 @@ __attribute__((amdgpu_waves_per_eu(D >= 256 ? 1 : D >= 128 ? 2 : 4))) paged_narr
       const int at = 2 * (s & 31) + hh, key = tile_of(s) * 32 + hh * kGranule;
       const uint32_t lds = wave_at + (values ? TILE_B : 0) + hh * GRAN_B;
       const char* base = (values ? vp : kp) + lane64(off, at);
-      const GranuleCopy<D>& c = values ? vc : kc;
+      const GranuleCopy<D, true>& c = values ? vc : kc;
       if (!((gr.live >> at) & 1)) c.zero(lds, lane);
       else if (key >= u.lo && key + kGranule <= end) c.whole(lds, base, ss_b);
       else c.part(lds, base, ss_b, max(0, u.lo - key), min(kGranule, end - key) - 1);
@@ -485,32 +476,106 @@ __attribute__((amdgpu_waves_per_eu(D >= 256 ? 1 : D >= 128 ? 2 : 4))) paged_narr
   }
 }
 
-// NW waves over tiles of BN keys in a ring of two. KG: waves that share the same 32 rows, each taking BN / KG keys of every
-// tile; a workgroup covers 32 * NW / KG rows. Each wave copies one granule of a tile (BN = 16 NW).
+// The stretch of narrow workgroup `wg`, segment by segment.
+template <typename T, int D, int NW, bool SOFTCAP>
+__device__ __forceinline__ void narrow_stretch(const PagedParams& p, const Division& d, char* smem, int hk, int wg) {
+  const int lane = threadIdx.x & 63;
+  const int from = wg * d.stretch, to = min(d.tiles, from + d.stretch);
+  for (int f = from; f < to;) {
+    Unit u;
+    u.row0 = 0;
+    int first, tiles, index;  // the segment's sequence: its first tile and their number, and its place in the slots
+    if (f < d.p_tiles) {
+      u.prefix = true;
+      u.b = 0;
+      u.s = Seq{0, 0, 0};
+      u.rows = p.T * p.G;
+      u.lo = d.p_lo;
+      u.hi = p.P;
+      first = index = 0;
+      tiles = d.p_tiles;
+    } else {
+      const Place pl = find_place<kNarrowTile>(p, d, f - d.p_tiles, lane);
+      if (pl.b < 0) return;
+      u.prefix = false;
+      u.b = pl.b;
+      u.s = pl.s;
+      u.rows = pl.s.n * p.G;
+      first = d.p_tiles + pl.tile0;
+      index = pl.b + (d.p_tiles > 0 ? 1 : 0);
+      set_range(p, u, kNarrowRows);
+      u.lo = first_key(p, u.s);
+      tiles = seq_tiles(p, u.s);
+    }
+    const int last = min(to, first + tiles);
+    const int t0 = u.lo / kTile;
+    u.k0 = (t0 + f - first) * kTile;
+    u.k1 = (t0 + last - first) * kTile;
+    u.whole = p.P == 0 && f == first && last == first + tiles;
+    use_slot<D>(p, u, false, wg + index, hk);
+    narrow_unit<T, D, NW, SOFTCAP>(p, u, smem, hk);
+    f = last;
+    if (f < to) __syncthreads();  // the states in the LDS are read
+  }
+}
+
+template <int D>
+__device__ __forceinline__ bool wide_unit_of(const PagedParams& p, const Division& d, int n, int hk, Unit& u) {
+  const int R = 1 << p.log2_r, p_units = d.p_rg * d.p_ns;
+  int k, ns, slot;
+  u.prefix = n < p_units;
+  if (u.prefix) {
+    k = n / d.p_rg;
+    const int rg = n - k * d.p_rg;
+    ns = d.p_ns;
+    u.b = 0;
+    u.s = Seq{0, 0, 0};
+    u.row0 = rg * R;
+    u.rows = p.T * p.G;
+    slot = rg * d.p_ns + k;
+    u.lo = d.p_lo;
+    u.hi = p.P;
+    u.whole = false;
+  } else {
+    const Place pl = find_place<kWideUnit>(p, d, n - p_units, threadIdx.x & 63);
+    if (pl.b < 0) return false;
+    const int nrg = row_groups(p, pl.s.n * p.G);
+    ns = wide_slices(p, pl.s, d);
+    k = pl.local / nrg;
+    const int rg = pl.local - k * nrg;
+    u.b = pl.b;
+    u.s = pl.s;
+    u.row0 = rg * R;
+    u.rows = pl.s.n * p.G;
+    slot = p_units + pl.slot0 + rg * ns + k;
+    u.whole = p.P == 0 && ns == 1;
+    set_range(p, u, R);
+  }
+  use_slot<D>(p, u, true, slot, hk);
+  const int tiles = key_tiles(u.lo, u.hi), per = ceil_div(tiles, ns), t0 = u.lo / kTile;
+  u.k0 = (t0 + min(tiles, k * per)) * kTile;
+  u.k1 = (t0 + min(tiles, (k + 1) * per)) * kTile;
+  return true;
+}
+
+// One wide unit: NW waves over tiles of BN keys in a ring of two. KG: waves that share the same 32 rows, each taking
+// BN / KG keys of every tile; a workgroup covers 32 * NW / KG rows. Each wave copies one granule of a tile (BN = 16 NW).
 template <typename T, int D, int NW, int KG, int OCC, bool SOFTCAP>
-__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
-paged_wide_kernel(PagedParams p) {
+__device__ __forceinline__ void wide_unit(const PagedParams& p, const Unit& u, char* smem, int hk) {
   typedef DmaLayout<D> L;
   typedef typename T::scalar S;
   typedef typename T::vec8 V8;
   typedef typename T::vec4 V4;
   constexpr int BN = kGranule * NW, SBN = BN / KG, NMB = SBN / 32, NWR = NW / KG;
   constexpr int TILE_B = (BN / L::GR) * L::GROUP_B, STAGE_B = 2 * TILE_B;
-  constexpr int GRAN_B = (kGranule / L::GR) * L::GROUP_B;
+  constexpr int GRAN_B = Lds<D, NW>::GRAN_B, SLOT_B = Lds<D, NW>::SLOT_B;
   constexpr int WINDOW = 64 / NW;                    // tiles whose granules the lanes hold
-  constexpr int SLOT_B = (D / 8) * kOQ;
-  constexpr int LOADS = GranuleCopy<D>::LOADS;
-  constexpr int SMEM_B = std::max(2 * STAGE_B, NW * (SLOT_B + 32 * 8));
+  constexpr int LOADS = GranuleCopy<D, false>::LOADS;
   static_assert(SBN % 32 == 0, "key groups");
-  __shared__ __attribute__((aligned(1024))) char smem[SMEM_B];
-
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = KG == 1 ? w : w % NWR, kg = KG == 1 ? 0 : w / NWR;
   const int koff = SBN * kg;
-  const int hk = blockIdx.y;
-  Unit u;
-  if (!find_unit(p, lane, u)) return;
 
   const int end = min(u.hi, u.k1);
   const int t_first = max(u.k0, u.lo) / BN, t_end = u.k1 > u.k0 ? ceil_div(end, BN) : t_first;
@@ -528,7 +593,7 @@ paged_wide_kernel(PagedParams p) {
 
   const uint32_t smem_at = (uint32_t)(size_t)((lds_char*)smem);
   const int64_t k_ss_b = 2 * p.k_ss, v_ss_b = 2 * p.v_ss;
-  GranuleCopy<D> kc, vc;
+  GranuleCopy<D, false> kc, vc;
   kc.init(lane, k_ss_b);
   vc.init(lane, v_ss_b);
   Fragments<D> fr;
@@ -703,152 +768,218 @@ paged_wide_kernel(PagedParams p) {
   }
 }
 
-// Joins the partials of rows: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, lse = (M + log2 L) ln 2, with the prefix
-// slices first and then the sequence's own. ROWS rows at a time per workgroup of 256: 256 / ROWS threads to a row, in
-// groups of D / 4 (four head-dim elements each) that take the slices in turn.
+constexpr int kNarrowWaves = 4;
+
+// Everything narrow. Waves per SIMD: as many workgroups per CU as the LDS holds (33 KiB at head_dim 64, 67 at 128, 133 at
+// 256).
+template <typename T, int D, bool SOFTCAP>
+__global__ void __launch_bounds__(64 * kNarrowWaves)
+__attribute__((amdgpu_waves_per_eu(D >= 256 ? 1 : D >= 128 ? 2 : 4))) paged_narrow_kernel(PagedParams p) {
+  __shared__ __attribute__((aligned(1024))) char smem[Lds<D, kNarrowWaves>::NARROW];
+  const int hk = blockIdx.x % p.Hkv, n = blockIdx.x / p.Hkv;
+  const Division d = divide(p, threadIdx.x & 63);
+  narrow_stretch<T, D, kNarrowWaves, SOFTCAP>(p, d, smem, hk, n);
+}
+
+// Wide units, then narrow stretches.
+template <typename T, int D, int NW, int KG, int OCC, bool SOFTCAP>
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
+paged_mixed_kernel(PagedParams p) {
+  __shared__ __attribute__((aligned(1024))) char smem[std::max(Lds<D, NW>::NARROW, Lds<D, NW>::WIDE)];
+  const int hk = blockIdx.x % p.Hkv, n = blockIdx.x / p.Hkv;
+  const Division d = divide(p, threadIdx.x & 63);
+  if (n >= p.wide_units) {
+    narrow_stretch<T, D, NW, SOFTCAP>(p, d, smem, hk, n - p.wide_units);
+    return;
+  }
+  Unit u;
+  if (wide_unit_of<D>(p, d, n, hk, u)) wide_unit<T, D, NW, KG, OCC, SOFTCAP>(p, u, smem, hk);
+}
+
+// Joins the partials of rows: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, lse = (M + log2 L) ln 2, with those of the
+// prefix first and then the sequence's own. A workgroup takes rows_per_merge rows of the batch (token-major, as the prefix
+// numbers them) of a KV head. Its groups of D / 4 threads (four head-dim elements each) take rows, or, where a row has many
+// partials, share one.
 constexpr int kMergeThreads = 256;
-template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(PagedParams p, int rows_per_wg) {
+template <typename T, int D>
+__global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(PagedParams p) {
   typedef typename T::scalar S;
   typedef typename T::vec4 V4;
-  constexpr int COLS = D / 4, NG = kMergeThreads / (COLS * ROWS);
-  static_assert(NG >= 1 && NG * COLS * ROWS == kMergeThreads, "threads");
-  __shared__ f32x4 part[ROWS][NG][COLS];
-  __shared__ f32x2 part_ml[ROWS][NG];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int hk = blockIdx.y;
-  const Division dv = divide(p, lane);
-  const Place pl = find_place<false>(p, dv, blockIdx.x, lane);
-  if (pl.b < 0 || (p.P == 0 && pl.ns == 1)) return;
-  const int rows = min(pl.s.n * p.G - pl.local * p.R, p.R);
-  const int slot0 = dv.p_rg * dv.p_ns + pl.slot + pl.local * pl.ns;
-  if (slot0 + pl.ns > p.slots) return;  // (only where cu_q descends)
-  const int col = tid % COLS, grp = tid / COLS % NG, rr = tid / (COLS * NG);
-  const int n_all = dv.p_ns + pl.ns;
-  const int64_t slot_rows = (int64_t)p.Hkv * p.rows_stride;
-  for (int r0 = blockIdx.z * rows_per_wg; r0 < min(rows, (int)(blockIdx.z + 1) * rows_per_wg); r0 += ROWS) {
-    const int rl = r0 + rr;
-    const bool ok = rl < rows;
-    const int row = pl.local * p.R + min(rl, rows - 1);
-    const int qi = row / p.G, qg = row - qi * p.G, tok = pl.s.t0 + qi, h = hk * p.G + qg;
-    const int prow = tok * p.G + qg, prg = prow / p.R, prl = prow - prg * p.R;
-    // partial i of this row: prefix slice i, or slice i - p_ns of the sequence
-    const int64_t own = ((int64_t)(slot0 - dv.p_ns) * p.Hkv + hk) * p.rows_stride + min(rl, rows - 1);
-    const int64_t pre = ((int64_t)prg * dv.p_ns * p.Hkv + hk) * p.rows_stride + prl;
-    float M = -INFINITY, Ls = 0.f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    constexpr int U = 4;  // partials in flight
-    for (int i0 = grp; i0 < n_all; i0 += NG * U) {
-      f32x4 o[U];
-      f32x2 x[U];
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const int i = min(i0 + NG * k, n_all - 1);
-        const int64_t at = (i < dv.p_ns ? pre : own) + i * slot_rows;
-        x[k] = *reinterpret_cast<const f32x2*>(p.part_ml + 2 * at);
-        o[k] = *reinterpret_cast<const f32x4*>(p.part_o + at * D + 4 * col);
-      }
-      float m = M;
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        if (i0 + NG * k >= n_all) x[k] = f32x2{-INFINITY, 0.f};
-        m = fmaxf(m, x[k][0]);
-      }
-      const float mu = m == -INFINITY ? 0.f : m, a = fast_exp2(M - mu);
-      acc *= a;
-      Ls *= a;
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const float wgt = fast_exp2(x[k][0] - mu);
-        acc += wgt * o[k];
-        Ls = fmaf(wgt, x[k][1], Ls);
-      }
-      M = m;
+  constexpr int COLS = D / 4, NG = kMergeThreads / COLS;
+  __shared__ f32x4 part[NG][COLS];
+  __shared__ f32x2 part_ml[NG];
+  const int tid = threadIdx.x, lane = tid & 63, col = tid % COLS, grp = tid / COLS;
+  const int hk = blockIdx.x % p.Hkv;
+  const int from = blockIdx.x / p.Hkv * p.rows_per_merge, to = min(p.T * p.G, from + p.rows_per_merge);
+  const Division d = divide(p, lane);
+  for (int f = from; f < to;) {
+    const Place pl = find_place<kToken>(p, d, f / p.G, lane);
+    if (pl.b < 0) return;  // behind the last sequence
+    const int r_from = pl.local * p.G + (f - f / p.G * p.G);  // rows of the sequence
+    const int r_to = min(pl.s.n * p.G, r_from + (to - f));
+    f += r_to - r_from;
+    // Its own partials: slots own0 + (wide: row group * ns) + 0 .. n_own - 1; the prefix's likewise.
+    const bool wide = is_wide(p, pl.s);
+    int n_own, own0;
+    if (wide) {
+      n_own = wide_slices(p, pl.s, d);
+      own0 = d.p_rg * d.p_ns + pl.slot0;
+    } else {
+      const int t0 = d.p_tiles + pl.tile0, t1 = t0 + seq_tiles(p, pl.s) - 1;
+      own0 = t0 / d.stretch;
+      n_own = t1 / d.stretch - own0 + 1;
+      own0 += pl.b + (d.p_tiles > 0 ? 1 : 0);
     }
-    if constexpr (NG > 1) {
-      part[rr][grp][col] = acc;
-      if (col == 0) part_ml[rr][grp] = f32x2{M, Ls};
-      __syncthreads();
-      if (grp == 0) {
-        M = -INFINITY;
+    const int n_pre = d.p_ns > 0 ? d.p_ns : d.p_tiles > 0 ? (d.p_tiles - 1) / d.stretch + 1 : 0;
+    const int n_all = n_pre + n_own;
+    if (p.P == 0 && n_own == 1) continue;  // written by its unit
+    const int last_slot = own0 + (wide ? (row_groups(p, pl.s.n * p.G) - 1) * n_own : 0) + n_own - 1;
+    if (last_slot >= (wide ? p.wide_slots : p.narrow_slots)) return;  // (only where cu_q descends)
+    int shared = 0;  // log2 of the groups that share a row
+    while ((1 << shared) < NG && (n_all >> shared) > 4 && (NG >> shared) > 1 &&
+           ((NG >> shared) > r_to - r_from || (n_all >> shared) > 8))
+      ++shared;
+    const int sub = grp & ((1 << shared) - 1), step = 1 << shared, rows_at_once = NG >> shared;
+    for (int r0 = r_from; r0 < r_to; r0 += rows_at_once) {
+      const int row = r0 + (grp >> shared);
+      const bool ok = row < r_to;
+      const int rc = min(row, r_to - 1);
+      const int qi = rc / p.G, qg = rc - qi * p.G, tok = pl.s.t0 + qi, h = hk * p.G + qg;
+      const int prow = tok * p.G + qg;
+      const float *pre_o, *pre_ml, *own_o, *own_ml;
+      int64_t pre_step, own_step;  // rows from one partial to the next
+      auto locate = [&](bool w, int slot, int rl, const float*& po, const float*& pm, int64_t& st) {
+        const int rows = w ? p.wide_rows : p.narrow_rows;
+        const int64_t at = ((int64_t)slot * p.Hkv + hk) * rows + rl;
+        st = (int64_t)p.Hkv * rows;
+        po = (w ? p.wide_o : p.narrow_o) + at * D + 4 * col;
+        pm = (w ? p.wide_ml : p.narrow_ml) + at * 2;
+      };
+      const int rg = rc >> p.log2_r, prg = prow >> p.log2_r, rmask = (1 << p.log2_r) - 1;
+      locate(wide, own0 + (wide ? rg * n_own : 0), wide ? rc & rmask : rc, own_o, own_ml, own_step);
+      locate(p.prefix_wide, p.prefix_wide ? prg * d.p_ns : 0, p.prefix_wide ? prow & rmask : prow, pre_o, pre_ml, pre_step);
+      float M = -INFINITY, Ls = 0.f;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      constexpr int U = 4;  // partials in flight
+      for (int i0 = sub; i0 < n_all; i0 += step * U) {
+        f32x4 o[U];
+        f32x2 x[U];
 #pragma unroll
-        for (int i = 0; i < NG; ++i) M = fmaxf(M, part_ml[rr][i][0]);
-        const float mu = M == -INFINITY ? 0.f : M;
-        Ls = 0.f;
-        acc = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-          const float wgt = fast_exp2(part_ml[rr][i][0] - mu);
-          Ls = fmaf(wgt, part_ml[rr][i][1], Ls);
-          acc += wgt * part[rr][i][col];
+        for (int k = 0; k < U; ++k) {
+          const int i = min(i0 + step * k, n_all - 1);
+          const bool pre = i < n_pre;
+          const int64_t at = pre ? i * pre_step : (i - n_pre) * own_step;
+          x[k] = *reinterpret_cast<const f32x2*>((pre ? pre_ml : own_ml) + 2 * at);
+          o[k] = *reinterpret_cast<const f32x4*>((pre ? pre_o : own_o) + at * D);
         }
-      }
-      __syncthreads();
-      if (grp != 0) continue;
-    }
-    if (!ok) continue;
-    const float inv = Ls == 0.f ? 0.f : 1.0f / Ls;
-    S* op = static_cast<S*>(p.o) + (p.cu_q != nullptr ? tok * p.o_ss : pl.b * p.o_sb + qi * p.o_ss) + h * p.o_sh;
-    V4 ov;
+        float m = M;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) ov[e] = to_s<S>(acc[e] * inv);
-    *reinterpret_cast<V4*>(op + 4 * col) = ov;
-    if (p.lse != nullptr && col == 0)
-      p.lse[(int64_t)tok * p.Hq + h] = Ls == 0.f ? -INFINITY : (M + fast_log2(Ls)) * kLn2;
+        for (int k = 0; k < U; ++k) {
+          if (i0 + step * k >= n_all) x[k] = f32x2{-INFINITY, 0.f};
+          m = fmaxf(m, x[k][0]);
+        }
+        const float mu = m == -INFINITY ? 0.f : m, a = fast_exp2(M - mu);
+        acc *= a;
+        Ls *= a;
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          const float wgt = fast_exp2(x[k][0] - mu);
+          acc += wgt * o[k];
+          Ls = fmaf(wgt, x[k][1], Ls);
+        }
+        M = m;
+      }
+      if (shared > 0) {
+        part[grp][col] = acc;
+        if (col == 0) part_ml[grp] = f32x2{M, Ls};
+        __syncthreads();
+        if (sub == 0) {
+          M = -INFINITY;
+          for (int i = 0; i < step; ++i) M = fmaxf(M, part_ml[grp + i][0]);
+          const float mu = M == -INFINITY ? 0.f : M;
+          Ls = 0.f;
+          acc = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int i = 0; i < step; ++i) {
+            const float wgt = fast_exp2(part_ml[grp + i][0] - mu);
+            Ls = fmaf(wgt, part_ml[grp + i][1], Ls);
+            acc += wgt * part[grp + i][col];
+          }
+        }
+        __syncthreads();
+      }
+      if (!ok || sub != 0) continue;
+      const float inv = Ls == 0.f ? 0.f : 1.0f / Ls;
+      S* op = static_cast<S*>(p.o) + (p.cu_q != nullptr ? tok * p.o_ss : pl.b * p.o_sb + qi * p.o_ss) + h * p.o_sh;
+      V4 ov;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ov[e] = to_s<S>(acc[e] * inv);
+      *reinterpret_cast<V4*>(op + 4 * col) = ov;
+      if (p.lse != nullptr && col == 0)
+        p.lse[(int64_t)tok * p.Hq + h] = Ls == 0.f ? -INFINITY : (M + fast_log2(Ls)) * kLn2;
+    }
   }
 }
 
 // The host's part of the division.
 struct HostPlan {
-  int R, rows_stride, target, min_slice, grid_units, slots, merge_units;
+  int log2_r, wide_target, wide_units, wide_slots, wide_rows, narrow_wgs, narrow_slots, narrow_rows, prefix_wide;
+  int64_t floats(int64_t Hkv, int64_t D) const {
+    return ((int64_t)wide_slots * wide_rows + (int64_t)narrow_slots * narrow_rows) * Hkv * (D + 2);
+  }
 };
+int env(const char* n, int d) { return getenv(n) ? atoi(getenv(n)) : d; }
 HostPlan host_plan(int64_t B, int64_t T, bool ragged, int64_t Hq, int64_t Hkv, int64_t D, int64_t P) {
   HostPlan h{};
-  const int64_t G = Hq / Hkv, Sq = B > 0 ? T / B : 0;
+  const int64_t G = Hq / Hkv, Sq = T / B;
   const int64_t most = (ragged ? T : Sq) * G;  // most rows that a sequence can have
-  // Rows that a workgroup finds to do: those of the average sequence (of the batch, where there is a prefix).
-  const int64_t typical = P > 0 ? T * G : ragged ? (T * G + B - 1) / B : most;
-  const int widest = D == 128 ? 256 : 128;
-  h.R = typical <= 32 ? 32 : typical <= 64 ? 64 : typical <= 128 || widest == 128 ? 128 : 256;
-  h.rows_stride = (int)std::min<int64_t>(h.R, P > 0 ? T * G : most);
-  h.target = (int)std::max<int64_t>(h.R == 32 ? 2048 : 768, Hkv);
-  h.min_slice = h.R == 32 ? 1 : 2;
-  const int64_t nrg = ragged ? T * G / h.R + std::min(B, T) : B * ((Sq * G + h.R - 1) / h.R);
-  const int64_t p_rg = P > 0 ? (T * G + h.R - 1) / h.R : 0;
-  h.merge_units = (int)nrg;
-  h.grid_units = (int)(h.target / Hkv + nrg + p_rg);
-  h.slots = P > 0 ? h.grid_units : (int)(2 * h.target / Hkv);
+  h.prefix_wide = P > 0 && T * G > dgg_paged::kNarrowRows;
+  const bool wide = most > dgg_paged::kNarrowRows || h.prefix_wide;
+  const bool narrow = ragged || Sq * G <= dgg_paged::kNarrowRows || (P > 0 && !h.prefix_wide);
+  if (wide) {
+    // Rows that a wide unit finds: those of the prefix, or of the average sequence that is wide, if half of them are.
+    const int64_t typical = h.prefix_wide ? T * G : ragged ? 2 * T * G / B : most;
+    const int widest = D == 128 ? 8 : 7;
+    h.log2_r = env("DGG_R", typical <= 64 ? 6 : typical <= 128 || widest == 7 ? 7 : 8);
+    h.wide_target = std::max<int>(1, env("DGG_T", 256) / Hkv);
+    const int64_t R = 1ll << h.log2_r;
+    // ragged: a sequence's rows fill row groups but for its last; only sequences of more than 32 rows count
+    const int64_t nrg = ragged ? T * G / R + std::min(B, T * G / (dgg_paged::kNarrowRows + 1))
+                               : most > dgg_paged::kNarrowRows ? B * ((most + R - 1) / R) : 0;
+    const int64_t p_rg = h.prefix_wide ? (T * G + R - 1) / R : 0;
+    h.wide_units = (int)(h.wide_target + nrg + p_rg);
+    h.wide_slots = P > 0 ? h.wide_units : 2 * h.wide_target;
+    h.wide_rows = (int)std::min<int64_t>(R, h.prefix_wide ? T * G : most);
+  }
+  if (narrow) {
+    h.narrow_wgs = std::max<int>(1, env("DGG_N", wide ? 256 : 512) / Hkv);
+    h.narrow_slots = (int)(h.narrow_wgs + B + 1);
+    h.narrow_rows = (int)std::min<int64_t>(dgg_paged::kNarrowRows, P > 0 && !h.prefix_wide ? T * G : most);
+  }
   return h;
 }
 
 template <typename T, int D, bool SOFTCAP>
-void launch_cap(const PagedParams& p, const HostPlan& h, hipStream_t st) {
-  const dim3 grid(h.grid_units, p.Hkv);
-  if (h.R == 32)
+void launch_cap(const PagedParams& p, hipStream_t st) {
+  const dim3 grid((unsigned)(p.wide_units + p.narrow_wgs) * p.Hkv);
+  if (p.wide_units == 0)
     hipLaunchKernelGGL((paged_narrow_kernel<T, D, SOFTCAP>), grid, dim3(64 * kNarrowWaves), 0, st, p);
   else if constexpr (D == 128) {
-    if (h.R == 64) hipLaunchKernelGGL((paged_wide_kernel<T, D, 8, 4, 2, SOFTCAP>), grid, dim3(512), 0, st, p);
-    else if (h.R == 128) hipLaunchKernelGGL((paged_wide_kernel<T, D, 8, 2, 2, SOFTCAP>), grid, dim3(512), 0, st, p);
-    else hipLaunchKernelGGL((paged_wide_kernel<T, D, 8, 1, 2, SOFTCAP>), grid, dim3(512), 0, st, p);
+    if (p.log2_r == 6) hipLaunchKernelGGL((paged_mixed_kernel<T, D, 8, 4, 2, SOFTCAP>), grid, dim3(512), 0, st, p);
+    else if (p.log2_r == 7) hipLaunchKernelGGL((paged_mixed_kernel<T, D, 8, 2, 2, SOFTCAP>), grid, dim3(512), 0, st, p);
+    else hipLaunchKernelGGL((paged_mixed_kernel<T, D, 8, 1, 2, SOFTCAP>), grid, dim3(512), 0, st, p);
   } else {
     constexpr int OCC = D == 64 ? 3 : 1;
-    if (h.R == 64) hipLaunchKernelGGL((paged_wide_kernel<T, D, 4, 2, OCC, SOFTCAP>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((paged_wide_kernel<T, D, 4, 1, OCC, SOFTCAP>), grid, dim3(256), 0, st, p);
+    if (p.log2_r == 6) hipLaunchKernelGGL((paged_mixed_kernel<T, D, 4, 2, OCC, SOFTCAP>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((paged_mixed_kernel<T, D, 4, 1, OCC, SOFTCAP>), grid, dim3(256), 0, st, p);
   }
 }
 template <typename T, int D>
-void launch(const PagedParams& p, const HostPlan& h, hipStream_t st) {
-  if (p.s.softcap > 0.f) launch_cap<T, D, true>(p, h, st);
-  else launch_cap<T, D, false>(p, h, st);
-  if (h.rows_stride <= 32) {
-    hipLaunchKernelGGL((paged_merge_kernel<T, D, 1>), dim3(h.merge_units, p.Hkv, h.rows_stride), dim3(kMergeThreads), 0,
-                       st, p, 1);
-  } else {
-    constexpr int ROWS = kMergeThreads / (D / 4);
-    const int rpw = 32;
-    hipLaunchKernelGGL((paged_merge_kernel<T, D, ROWS>), dim3(h.merge_units, p.Hkv, (h.rows_stride + rpw - 1) / rpw),
-                       dim3(kMergeThreads), 0, st, p, rpw);
-  }
+void launch(const PagedParams& p, hipStream_t st) {
+  if (p.s.softcap > 0.f) launch_cap<T, D, true>(p, st);
+  else launch_cap<T, D, false>(p, st);
+  const int64_t rows = (int64_t)p.T * p.G;
+  const int64_t wgs = (rows + p.rows_per_merge - 1) / p.rows_per_merge * p.Hkv;
+  hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3((unsigned)wgs), dim3(kMergeThreads), 0, st, p);
 }
 
 int check_sizes(const char* op, int64_t B, int64_t T, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix) {
@@ -858,7 +989,8 @@ int check_sizes(const char* op, int64_t B, int64_t T, int64_t Sq, int64_t Hq, in
               (long long)T, (long long)B, (long long)Sq);
   DGG_REQUIRE(Hq > 0 && Hkv > 0 && Hq <= 1024 && Hq % Hkv == 0, DGG_ERR_SHAPE, "%s: bad head counts (Hq=%lld Hkv=%lld)",
               op, (long long)Hq, (long long)Hkv);
-  DGG_REQUIRE(T * (Hq / Hkv) < (1 << 30), DGG_ERR_SHAPE, "%s: too many query rows", op);
+  DGG_REQUIRE(T * Hq < (1 << 28), DGG_ERR_SHAPE, "%s: too many query rows (%lld tokens of %lld heads)", op, (long long)T,
+              (long long)Hq);
   DGG_REQUIRE(D == 64 || D == 128 || D == 256, DGG_ERR_UNSUPPORTED, "%s: head_dim %lld not supported (64, 128, 256)",
               op, (long long)D);
   DGG_REQUIRE(prefix >= 0, DGG_ERR_SHAPE, "%s: prefix_len must be >= 0 (got %lld)", op, (long long)prefix);
@@ -871,8 +1003,7 @@ extern "C" int64_t dgg_attn_paged_workspace_bytes(int64_t B, int64_t T, int64_t 
                                                   int64_t prefix_len) {
   if (check_sizes("attn_paged_workspace_bytes", B, T, Sq, Hq, Hkv, D, prefix_len)) return -1;
   if (B == 0 || T == 0) return 0;
-  const HostPlan h = host_plan(B, T, Sq == 0, Hq, Hkv, D, prefix_len);
-  return (int64_t)h.slots * Hkv * h.rows_stride * (D + 2) * (int64_t)sizeof(float);
+  return host_plan(B, T, Sq == 0, Hq, Hkv, D, prefix_len).floats(Hkv, D) * (int64_t)sizeof(float);
 }
 
 extern "C" int dgg_attn_paged(const void* q, const void* k_pages, const void* v_pages, void* o, float* lse,
@@ -895,6 +1026,7 @@ extern "C" int dgg_attn_paged(const void* q, const void* k_pages, const void* v_
   DGG_REQUIRE(table_width >= 0 && table_width * page_size < (1ll << 30), DGG_ERR_SHAPE,
               "%s: a block table row of %lld pages of %lld is too long", op, (long long)table_width,
               (long long)page_size);
+  DGG_REQUIRE(B * table_width * page_size < (1ll << 37), DGG_ERR_SHAPE, "%s: a block table of more than 2^37 keys", op);
   DGG_REQUIRE(prefix_len % page_size == 0 && prefix_len <= table_width * page_size, DGG_ERR_SHAPE,
               "%s: prefix_len %lld must be whole pages of the block table", op, (long long)prefix_len);
   DGG_REQUIRE(std::isfinite(scale) && scale > 0.f, DGG_ERR_SHAPE, "%s: scale must be finite and > 0", op);
@@ -932,8 +1064,17 @@ extern "C" int dgg_attn_paged(const void* q, const void* k_pages, const void* v_
   p.table = block_table;
   p.kv_lens = kv_lens;
   p.cu_q = Sq > 0 ? nullptr : cu_q;
-  p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o + (int64_t)h.slots * Hkv * h.rows_stride * D;
+  float* ws = static_cast<float*>(workspace);
+  auto carve = [&](int64_t n) {
+    float* at = ws;
+    ws += n;
+    return at;
+  };
+  const int64_t wide_all = (int64_t)h.wide_slots * h.wide_rows * Hkv, narrow_all = (int64_t)h.narrow_slots * h.narrow_rows * Hkv;
+  p.wide_o = carve(wide_all * D);
+  p.narrow_o = carve(narrow_all * D);
+  p.wide_ml = carve(wide_all * 2);
+  p.narrow_ml = carve(narrow_all * 2);
   p.q_sb = strides[0]; p.q_ss = strides[1]; p.q_sh = strides[2];
   p.k_sp = strides[3]; p.k_ss = strides[4]; p.k_sh = strides[5];
   p.v_sp = strides[6]; p.v_ss = strides[7]; p.v_sh = strides[8];
@@ -951,21 +1092,25 @@ extern "C" int dgg_attn_paged(const void* q, const void* k_pages, const void* v_
   p.P = (int)std::min(prefix_len, cap);
   p.causal = (flags & DGG_ATTN_CAUSAL) != 0;
   p.window = (int)std::min<int64_t>(window, 1 << 30);
-  p.R = h.R;
-  p.rows_stride = h.rows_stride;
-  p.min_slice = h.min_slice;
-  p.per_target = (float)((1.0 + 1.0 / 2048) * (double)Hkv / (double)h.target);
-  p.grid_units = h.grid_units;
-  p.slots = h.slots;
+  p.log2_r = h.log2_r;
+  p.prefix_wide = h.prefix_wide;
+  p.wide_units = h.wide_units;
+  p.wide_slots = h.wide_slots;
+  p.wide_rows = h.wide_rows;
+  p.narrow_wgs = h.narrow_wgs;
+  p.narrow_slots = h.narrow_slots;
+  p.narrow_rows = h.narrow_rows;
+  p.per_wide = h.wide_target > 0 ? (float)((1.0 + 1.0 / 2048) / h.wide_target) : 0.f;
+  p.rows_per_merge = (int)std::max<int64_t>(1, T * p.G * Hkv / 2048);
   hipStream_t st = dgg::as_stream(stream);
   if (dtype == DGG_BF16) {
-    if (D == 64) launch<BF16, 64>(p, h, st);
-    else if (D == 128) launch<BF16, 128>(p, h, st);
-    else launch<BF16, 256>(p, h, st);
+    if (D == 64) launch<BF16, 64>(p, st);
+    else if (D == 128) launch<BF16, 128>(p, st);
+    else launch<BF16, 256>(p, st);
   } else {
-    if (D == 64) launch<F16, 64>(p, h, st);
-    else if (D == 128) launch<F16, 128>(p, h, st);
-    else launch<F16, 256>(p, h, st);
+    if (D == 64) launch<F16, 64>(p, st);
+    else if (D == 128) launch<F16, 128>(p, st);
+    else launch<F16, 256>(p, st);
   }
   return dgg::check_launch(op);
 }
