@@ -48,6 +48,7 @@ struct PagedParams {
   int64_t table_sb;
   int B, T, Sq, Hq, Hkv, G;
   int num_pages, gpp, cap;  // pages, granules per page, keys that a table row can name
+  uint32_t gpp_mul, gpp_shift;  // page_index
   int P;                    // shared prefix (a multiple of the page size)
   int causal, window;
   int log2_r;               // row group of wide units
@@ -61,6 +62,12 @@ struct PagedParams {
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// gi / gpp for gi < 2^26 (the quotient of a number of 32 bits by multiplication: gpp_mul = ceil(2^(32 + shift) / gpp) is
+// off by less than gpp * 2^-(32 + shift) of it, and shift is at least log2(gpp) - 6).
+__device__ __forceinline__ int page_index(const PagedParams& p, int gi) {
+  return p.gpp == 1 ? gi : (int)(__umulhi((uint32_t)gi, p.gpp_mul) >> p.gpp_shift);
+}
 
 struct Seq {
   int t0, n, kv;  // first token, tokens, keys

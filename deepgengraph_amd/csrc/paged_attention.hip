@@ -29,6 +29,14 @@ namespace {
 using namespace dgg_attn;
 using namespace dgg_paged;
 
+// The launch parameters, read from the kernel's arguments anew: a part of the kernel that begins with this does not keep
+// scalar registers for what other parts use (without it 80 to 150 of them spill).
+__device__ __forceinline__ const PagedParams& fresh_params() {
+  auto at = (const PagedParams __attribute__((address_space(4)))*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(at));
+  return *(const PagedParams*)at;
+}
+
 // A unit of work: rows and keys.
 struct Unit {
   bool prefix;
@@ -112,33 +120,29 @@ __device__ __forceinline__ Seen seen_by_wave(const Row& x) {
   return v;
 }
 
-// Where 64 granules are, one per lane: byte offsets of their first K and V row, and which of them hold a key of the unit.
-// The page numbers of the next 64 are requested when these are taken up, so that their latency is not waited for.
+// The pages of 64 granules, one per lane, and which of the granules hold a key of the unit. The page numbers of the next 64
+// are requested when these are taken up, so that their latency is not waited for.
 struct Granules {
   const int32_t* row;  // the sequence's row of the table
-  int64_t ko, vo;
-  int next;            // page number of the granule that comes next
+  int page, next;
   uint64_t live;       // bit l: the granule of lane l holds a key
   __device__ __forceinline__ int page_of(const PagedParams& p, int gi) {
-    return row[min(gi, p.cap / kGranule - 1) / p.gpp];
+    return row[page_index(p, min(gi, p.cap / kGranule - 1))];
   }
   // Takes up granule gi (per lane) with its page number in `next`, and requests that of gi_next.
   __device__ __forceinline__ void take(const PagedParams& p, const Unit& u, int gi, int gi_next) {
-    const int page = next;
+    page = next;
     next = page_of(p, gi_next);
     const int key = gi * kGranule;
-    const bool ok = page >= 0 && page < p.num_pages && key + kGranule > u.lo && key < min(u.hi, u.k1);
-    const int in = (gi % p.gpp) * kGranule;
-    ko = 2 * (page * p.k_sp + in * p.k_ss);
-    vo = 2 * (page * p.v_sp + in * p.v_ss);
-    live = __ballot(ok);
+    live = __ballot(page >= 0 && page < p.num_pages && key + kGranule > u.lo && key < min(u.hi, u.k1));
+  }
+  // Byte offset of the first row of granule gi, which lane `at` holds.
+  __device__ __forceinline__ int64_t offset(const PagedParams& p, int gi, int at, int64_t sp, int64_t ss) const {
+    const int pg = __builtin_amdgcn_readlane(page, at);
+    const int in = (gi - page_index(p, gi) * p.gpp) * kGranule;
+    return 2 * (pg * sp + in * ss);
   }
 };
-__device__ __forceinline__ int64_t lane64(int64_t x, int at) {
-  const unsigned lo32 = __builtin_amdgcn_readlane((int)(x & 0xffffffff), at);
-  const int hi32 = __builtin_amdgcn_readlane((int)(x >> 32), at);
-  return (int64_t)hi32 << 32 | lo32;
-}
 
 // dma16 (attention_common.h), with the non-temporal hint for NT: rows that one workgroup reads once.
 template <bool NT>
@@ -157,19 +161,19 @@ struct GranuleCopy {
   typedef DmaLayout<D> L;
   static constexpr int LOADS = kGranule / L::RPI;  // direct loads per granule
   uint32_t voff[L::NV];  // lane constants: row within the load's group, and the chunk that the layout puts there
-  uint32_t chunk[L::NV];
-  int lrow;
   // D == 64: the swizzle depends on the 8-row group's number, whose parity is that of the load within the granule.
   static __device__ __forceinline__ int vi(int i) { return D == 64 ? i & 1 : i % L::IPG; }
   __device__ __forceinline__ void init(int lane, int64_t ss_b) {
-    lrow = lane / L::LPR;
+    const int lrow = lane / L::LPR;
 #pragma unroll
     for (int i = 0; i < L::NV; ++i) {
-      const int trow = i * L::RPI + lrow;  // (row within a granule, which is all that the swizzle looks at)
-      chunk[i] = (uint32_t)((lane % L::LPR) ^ L::swizzle(trow)) * 16u;
-      voff[i] = (uint32_t)((D == 64 ? lrow : trow) * ss_b) + chunk[i];
+      voff[i] = (uint32_t)((D == 64 ? lrow : i * L::RPI + lrow) * ss_b) + chunk(lane, i);
       asm volatile("" : "+v"(voff[i]));
     }
+  }
+  // (the swizzle looks at the row within a granule only)
+  static __device__ __forceinline__ uint32_t chunk(int lane, int i) {
+    return (uint32_t)((lane % L::LPR) ^ L::swizzle(i * L::RPI + lane / L::LPR)) * 16u;
   }
   static __device__ __forceinline__ uint32_t place(int i) {
     return (uint32_t)((i / L::IPG) * L::GROUP_B + (i % L::IPG) * L::RPI * L::ROW_B);
@@ -181,11 +185,11 @@ struct GranuleCopy {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) one(lds, base, ss_b, i);
   }
-  __device__ __forceinline__ void part(uint32_t lds, const char* base, int64_t ss_b, int first, int last) const {
+  static __device__ __forceinline__ void part(uint32_t lds, const char* base, int64_t ss_b, int first, int last, int lane) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int row = clampi(i * L::RPI + lrow, first, last);
-      dma16(lds + place(i), base + (row * ss_b + chunk[vi(i)]));
+      const int row = clampi(i * L::RPI + lane / L::LPR, first, last);
+      dma16(lds + place(i), base + (row * ss_b + chunk(lane, vi(i))));
     }
   }
   static __device__ __forceinline__ void zero(uint32_t lds, int lane) {
@@ -337,14 +341,17 @@ struct Lds {
 
 // One narrow unit: its keys over NW waves.
 template <typename T, int D, int NW, bool SOFTCAP>
-__device__ __forceinline__ void narrow_unit(const PagedParams& p, const Unit& u, char* smem, int hk) {
+__device__ __forceinline__ void narrow_unit(const Unit& u, char* smem, int hk) {
   typedef DmaLayout<D> L;
   typedef typename T::scalar S;
   typedef typename T::vec8 V8;
   typedef typename T::vec4 V4;
   constexpr int TILE_B = Lds<D, NW>::TILE_B, GRAN_B = Lds<D, NW>::GRAN_B, WAVE_B = Lds<D, NW>::WAVE_B;
   constexpr int LOADS = 2 * GranuleCopy<D, true>::LOADS;   // direct loads of a tile, K or V
-  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
+  const PagedParams& p = fresh_params();
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));  // the lane constants are made anew for each unit: kept over all of them, they spill
+  const int lane = tid & 63, r = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   // The wave's tiles: every NW-th of the slice's 32-key tiles that hold a key.
@@ -375,16 +382,17 @@ __device__ __forceinline__ void narrow_unit(const PagedParams& p, const Unit& u,
   // Copies the K (V) rows of own tile s to the wave's K (V) buffer.
   const int end = min(u.hi, u.k1);
   auto copy = [&](int s, bool values) {
-    const int64_t off = values ? gr.vo : gr.ko, ss_b = values ? v_ss_b : k_ss_b;
+    const int64_t ss_b = values ? v_ss_b : k_ss_b;
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
       const int at = 2 * (s & 31) + hh, key = tile_of(s) * 32 + hh * kGranule;
       const uint32_t lds = wave_at + (values ? TILE_B : 0) + hh * GRAN_B;
-      const char* base = (values ? vp : kp) + lane64(off, at);
+      const char* base = values ? vp + gr.offset(p, key / kGranule, at, p.v_sp, p.v_ss)
+                                : kp + gr.offset(p, key / kGranule, at, p.k_sp, p.k_ss);
       const GranuleCopy<D, true>& c = values ? vc : kc;
       if (!((gr.live >> at) & 1)) c.zero(lds, lane);
       else if (key >= u.lo && key + kGranule <= end) c.whole(lds, base, ss_b);
-      else c.part(lds, base, ss_b, max(0, u.lo - key), min(kGranule, end - key) - 1);
+      else c.part(lds, base, ss_b, max(0, u.lo - key), min(kGranule, end - key) - 1, lane);
     }
   };
   auto holes_of = [&](int s) { return ~(unsigned)(gr.live >> (2 * (s & 31))) & 3u; };
@@ -467,21 +475,22 @@ __device__ __forceinline__ void narrow_unit(const PagedParams& p, const Unit& u,
   wait_vmem<0>();
   put_state(st, slots + w * WAVE_B, ml + 32 * w, c, lane);
   __syncthreads();
+  const PagedParams& pe = fresh_params();
   const int live_rows = min(32, u.rows - u.row0);
   for (int it = tid; it < live_rows * (D / 8); it += 64 * NW) {
     const int row = it / (D / 8), quad = it % (D / 8);
-    const Row y = find_row(p, u, row, hk);
+    const Row y = find_row(pe, u, row, hk);
     if (!y.ok) continue;
-    write_row<T, D, NW>(p, u, slots, ml, 1, WAVE_B, row, quad, y.o, (int64_t)y.tok * p.Hq + y.h, row, hk);
+    write_row<T, D, NW>(pe, u, slots, ml, 1, WAVE_B, row, quad, y.o, (int64_t)y.tok * pe.Hq + y.h, row, hk);
   }
 }
 
 // The stretch of narrow workgroup `wg`, segment by segment.
 template <typename T, int D, int NW, bool SOFTCAP>
-__device__ __forceinline__ void narrow_stretch(const PagedParams& p, const Division& d, char* smem, int hk, int wg) {
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ void narrow_stretch(const Division& d, char* smem, int hk, int wg) {
   const int from = wg * d.stretch, to = min(d.tiles, from + d.stretch);
   for (int f = from; f < to;) {
+    const PagedParams& p = fresh_params();
     Unit u;
     u.row0 = 0;
     int first, tiles, index;  // the segment's sequence: its first tile and their number, and its place in the slots
@@ -495,6 +504,8 @@ __device__ __forceinline__ void narrow_stretch(const PagedParams& p, const Divis
       first = index = 0;
       tiles = d.p_tiles;
     } else {
+      int lane = threadIdx.x & 63;
+      asm volatile("" : "+v"(lane));
       const Place pl = find_place<kNarrowTile>(p, d, f - d.p_tiles, lane);
       if (pl.b < 0) return;
       u.prefix = false;
@@ -513,7 +524,7 @@ __device__ __forceinline__ void narrow_stretch(const PagedParams& p, const Divis
     u.k1 = (t0 + last - first) * kTile;
     u.whole = p.P == 0 && f == first && last == first + tiles;
     use_slot<D>(p, u, false, wg + index, hk);
-    narrow_unit<T, D, NW, SOFTCAP>(p, u, smem, hk);
+    narrow_unit<T, D, NW, SOFTCAP>(u, smem, hk);
     f = last;
     if (f < to) __syncthreads();  // the states in the LDS are read
   }
@@ -561,7 +572,7 @@ __device__ __forceinline__ bool wide_unit_of(const PagedParams& p, const Divisio
 // One wide unit: NW waves over tiles of BN keys in a ring of two. KG: waves that share the same 32 rows, each taking
 // BN / KG keys of every tile; a workgroup covers 32 * NW / KG rows. Each wave copies one granule of a tile (BN = 16 NW).
 template <typename T, int D, int NW, int KG, int OCC, bool SOFTCAP>
-__device__ __forceinline__ void wide_unit(const PagedParams& p, const Unit& u, char* smem, int hk) {
+__device__ __forceinline__ void wide_unit(const Unit& u, char* smem, int hk) {
   typedef DmaLayout<D> L;
   typedef typename T::scalar S;
   typedef typename T::vec8 V8;
@@ -572,6 +583,7 @@ __device__ __forceinline__ void wide_unit(const PagedParams& p, const Unit& u, c
   constexpr int WINDOW = 64 / NW;                    // tiles whose granules the lanes hold
   constexpr int LOADS = GranuleCopy<D, false>::LOADS;
   static_assert(SBN % 32 == 0, "key groups");
+  const PagedParams& p = fresh_params();
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = KG == 1 ? w : w % NWR, kg = KG == 1 ? 0 : w / NWR;
@@ -613,8 +625,8 @@ __device__ __forceinline__ void wide_unit(const PagedParams& p, const Unit& u, c
       gr.take(p, u, gran_of(t), gran_of(t + WINDOW));
     }
     const int at = (t - w_tile) * NW + w;
-    kb = kp + lane64(gr.ko, at);
-    vb = vp + lane64(gr.vo, at);
+    kb = kp + gr.offset(p, t * NW + w, at, p.k_sp, p.k_ss);
+    vb = vp + gr.offset(p, t * NW + w, at, p.v_sp, p.v_ss);
     g_key = t * BN + w * kGranule;
     g_live = (gr.live >> at) & 1;
     g_whole = g_live && g_key >= u.lo && g_key + kGranule <= end;
@@ -630,8 +642,8 @@ __device__ __forceinline__ void wide_unit(const PagedParams& p, const Unit& u, c
       vc.whole(dst + TILE_B, vb, v_ss_b);
     } else {
       const int first = max(0, u.lo - g_key), last = min(kGranule, end - g_key) - 1;
-      kc.part(dst, kb, k_ss_b, first, last);
-      vc.part(dst + TILE_B, vb, v_ss_b, first, last);
+      kc.part(dst, kb, k_ss_b, first, last, lane);
+      vc.part(dst + TILE_B, vb, v_ss_b, first, last, lane);
     }
   };
 
@@ -737,19 +749,33 @@ __device__ __forceinline__ void wide_unit(const PagedParams& p, const Unit& u, c
     }
   };
 
-  for (int t = t_first; t < t_end; ++t) {
-    wait_vmem<0>();
-    __syncthreads();
-    const unsigned holes = next_holes;
-    const int kb0 = t * BN + koff;
-    const bool more = t + 1 < t_end;
+  // Runs of full tiles and of others, in loops of their own (one loop with both would copy O from one's registers to the
+  // other's in every tile). look: the kind of tile t, and the granule copied during it.
+  unsigned holes = 0;
+  bool more = false, full = false;
+  auto look = [&](int t) __attribute__((always_inline)) {
+    holes = next_holes;
+    more = t + 1 < t_end;
     if (more) aim(t + 1);
-    const bool full = holes == 0 && kb0 >= see.lo_max && kb0 + SBN - 1 <= see.hi_min;
-    if (full && more && g_whole) {
+    const int kb0 = t * BN + koff;
+    full = more && g_whole && holes == 0 && kb0 >= see.lo_max && kb0 + SBN - 1 <= see.hi_min;
+  };
+  int t = t_first;
+  if (t < t_end) look(t);
+  while (t < t_end) {
+    while (t < t_end && full) {
+      wait_vmem<0>();
+      __syncthreads();
       tile(t, 0, std::false_type{});
-    } else {
+      if (++t < t_end) look(t);
+    }
+    while (t < t_end && !full) {
+      wait_vmem<0>();
+      __syncthreads();
       if (more) issue(t + 1);
+      const int kb0 = t * BN + koff;
       if (kb0 <= see.hi_max && kb0 + SBN - 1 >= see.lo_min) tile(t, holes, std::true_type{});
+      if (++t < t_end) look(t);
     }
   }
 
@@ -758,13 +784,14 @@ __device__ __forceinline__ void wide_unit(const PagedParams& p, const Unit& u, c
   __syncthreads();  // every wave is done with the tiles
   put_state(st, smem + w * SLOT_B, ml + 32 * w, c, lane);
   __syncthreads();
+  const PagedParams& pe = fresh_params();
   const int live_rows = min(32 * NWR, u.rows - u.row0);
   for (int it = tid; it < live_rows * (D / 8); it += 64 * NW) {
     const int row = it / (D / 8), quad = it % (D / 8);
-    const Row y = find_row(p, u, row, hk);
+    const Row y = find_row(pe, u, row, hk);
     if (!y.ok) continue;
-    write_row<T, D, KG>(p, u, smem + (row / 32) * SLOT_B, ml + 32 * (row / 32), NWR, SLOT_B, row % 32, quad, y.o,
-                        (int64_t)y.tok * p.Hq + y.h, row, hk);
+    write_row<T, D, KG>(pe, u, smem + (row / 32) * SLOT_B, ml + 32 * (row / 32), NWR, SLOT_B, row % 32, quad, y.o,
+                        (int64_t)y.tok * pe.Hq + y.h, row, hk);
   }
 }
 
@@ -778,22 +805,22 @@ __attribute__((amdgpu_waves_per_eu(D >= 256 ? 1 : D >= 128 ? 2 : 4))) paged_narr
   __shared__ __attribute__((aligned(1024))) char smem[Lds<D, kNarrowWaves>::NARROW];
   const int hk = blockIdx.x % p.Hkv, n = blockIdx.x / p.Hkv;
   const Division d = divide(p, threadIdx.x & 63);
-  narrow_stretch<T, D, kNarrowWaves, SOFTCAP>(p, d, smem, hk, n);
+  narrow_stretch<T, D, kNarrowWaves, SOFTCAP>(d, smem, hk, n);
 }
 
-// Wide units, then narrow stretches.
+// Narrow stretches, then wide units.
 template <typename T, int D, int NW, int KG, int OCC, bool SOFTCAP>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
 paged_mixed_kernel(PagedParams p) {
   __shared__ __attribute__((aligned(1024))) char smem[std::max(Lds<D, NW>::NARROW, Lds<D, NW>::WIDE)];
   const int hk = blockIdx.x % p.Hkv, n = blockIdx.x / p.Hkv;
   const Division d = divide(p, threadIdx.x & 63);
-  if (n >= p.wide_units) {
-    narrow_stretch<T, D, NW, SOFTCAP>(p, d, smem, hk, n - p.wide_units);
+  if (n < p.narrow_wgs) {
+    narrow_stretch<T, D, NW, SOFTCAP>(d, smem, hk, n);
     return;
   }
   Unit u;
-  if (wide_unit_of<D>(p, d, n, hk, u)) wide_unit<T, D, NW, KG, OCC, SOFTCAP>(p, u, smem, hk);
+  if (wide_unit_of<D>(p, d, n - p.narrow_wgs, hk, u)) wide_unit<T, D, NW, KG, OCC, SOFTCAP>(u, smem, hk);
 }
 
 // Joins the partials of rows: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, lse = (M + log2 L) ln 2, with those of the
@@ -1089,6 +1116,10 @@ extern "C" int dgg_attn_paged(const void* q, const void* k_pages, const void* v_
   p.num_pages = (int)num_pages;
   p.gpp = (int)(page_size / dgg_paged::kGranule);
   p.cap = (int)cap;
+  int log2_up = 0;
+  while ((1 << log2_up) < p.gpp) ++log2_up;
+  p.gpp_shift = (uint32_t)std::max(0, log2_up - 6);
+  p.gpp_mul = p.gpp == 1 ? 0 : (uint32_t)(((1ull << (32 + p.gpp_shift)) + p.gpp - 1) / p.gpp);
   p.P = (int)std::min(prefix_len, cap);
   p.causal = (flags & DGG_ATTN_CAUSAL) != 0;
   p.window = (int)std::min<int64_t>(window, 1 << 30);
