@@ -127,7 +127,8 @@ __device__ __forceinline__ float wave_sum_f(float x) {
   })));
 }
 
-// What every wave finds out from all the lengths.
+// What every wave finds out from all the lengths. Lane l looks at sequences l * c .. l * c + c - 1 (c = ceil(B / 64)); what
+// it found is kept, so that looking up a sequence later takes a ballot and not a second look at the lengths.
 struct Division {
   int slice;         // most key tiles of a wide unit
   int p_lo;          // first prefix key that any row sees
@@ -135,38 +136,58 @@ struct Division {
   int p_tiles;       // narrow prefix: tiles
   int stretch;       // tiles of a narrow workgroup
   int tiles;         // all narrow tiles
+  // per lane: the last of its sequences, and its own and the running number of narrow tiles, wide units, partial slots
+  Seq s;
+  int my_tiles, my_units, my_slots, run_tiles, run_units, run_slots;
 };
 __device__ __forceinline__ int seq_tiles(const PagedParams& p, const Seq& s) {
   return max(1, key_tiles(first_key(p, s), s.kv));  // (a sequence without keys has an output, too)
 }
+__device__ __forceinline__ int wide_slices(const PagedParams& p, const Seq& s, int slice) {
+  return ceil_div(seq_tiles(p, s), slice);
+}
+// Narrow tiles of a sequence, its wide units and their partial slots.
+template <bool WIDE>
+__device__ __forceinline__ void count_seq(const PagedParams& p, const Seq& s, int slice, int& tiles, int& units, int& slots) {
+  tiles = units = slots = 0;
+  if (s.n == 0) return;
+  if (!is_wide(p, s)) {
+    tiles = seq_tiles(p, s);
+  } else if constexpr (WIDE) {
+    const int ns = wide_slices(p, s, slice);
+    units = row_groups(p, s.n * p.G) * ns;
+    slots = p.P > 0 || ns > 1 ? units : 0;
+  }
+}
+// WIDE false: nothing of the launch is wide.
+template <bool WIDE>
 __device__ __forceinline__ Division divide(const PagedParams& p, int lane) {
   const int c = (p.B + 63) >> 6;
   float work = 0.f;  // (32 bits do: the quotient is rounded up, and every wave adds in the same order)
-  int narrow = 0, lo = p.P;
+  int lo = p.P;
+  Division d{};
   for (int j = 0; j < c; ++j) {
     const int b = lane * c + j;
     if (b >= p.B) break;
-    const Seq s = load_seq(p, b);
-    if (s.n == 0) continue;
-    if (is_wide(p, s)) work += (float)row_groups(p, s.n * p.G) * (float)seq_tiles(p, s);
-    else narrow += seq_tiles(p, s);
-    lo = min(lo, p.window > 0 ? max(0, s.kv - s.n - p.window + 1) : 0);
+    d.s = load_seq(p, b);
+    if (d.s.n == 0) continue;
+    if (!is_wide(p, d.s)) d.my_tiles += seq_tiles(p, d.s);
+    else if (WIDE) work += (float)row_groups(p, d.s.n * p.G) * (float)seq_tiles(p, d.s);
+    lo = min(lo, p.window > 0 ? max(0, d.s.kv - d.s.n - p.window + 1) : 0);
   }
-  Division d{};
   int p_tiles = 0;
   if (p.P > 0) {
     d.p_lo = wave_min_i(lo);
     p_tiles = key_tiles(d.p_lo, p.P);
   }
-  if (p.narrow_wgs > 0) {
-    d.tiles = last_lane(wave_scan_add(narrow));
-    if (!p.prefix_wide) {
-      d.p_tiles = p_tiles;
-      d.tiles += p_tiles;
-    }
-    d.stretch = ceil_div(d.tiles, p.narrow_wgs);
+  d.run_tiles = wave_scan_add(d.my_tiles);
+  d.tiles = last_lane(d.run_tiles);
+  if (!WIDE || !p.prefix_wide) {
+    d.p_tiles = p_tiles;
+    d.tiles += p_tiles;
   }
-  if (p.wide_units > 0) {
+  d.stretch = p.narrow_wgs > 0 ? ceil_div(d.tiles, p.narrow_wgs) : 0;
+  if constexpr (WIDE) {
     work = wave_sum_f(work);
     if (p.prefix_wide) {
       d.p_rg = row_groups(p, p.T * p.G);
@@ -174,7 +195,22 @@ __device__ __forceinline__ Division divide(const PagedParams& p, int lane) {
     }
     // At least work / wide_target: the sum of 4096 terms in fp32 is off by less than 2^-12 of it.
     d.slice = max(1, (int)ceilf(min(work * p.per_wide, 1e9f)));
-    d.p_ns = ceil_div(d.p_rg > 0 ? p_tiles : 0, d.slice);
+    if (d.p_rg > 0) d.p_ns = ceil_div(p_tiles, d.slice);
+    if (c == 1) {
+      if (lane < p.B) {
+        int tiles;
+        count_seq<WIDE>(p, d.s, d.slice, tiles, d.my_units, d.my_slots);
+      }
+    } else {
+      for (int j = 0; j < c && lane * c + j < p.B; ++j) {
+        int tiles, units, slots;
+        count_seq<WIDE>(p, load_seq(p, lane * c + j), d.slice, tiles, units, slots);
+        d.my_units += units;
+        d.my_slots += slots;
+      }
+    }
+    d.run_units = wave_scan_add(d.my_units);
+    d.run_slots = wave_scan_add(d.my_slots);
   }
   return d;
 }
@@ -188,74 +224,64 @@ struct Place {
   int tile0;   // narrow tiles before it
   int slot0;   // wide partial slots before it (behind the prefix's)
 };
-__device__ __forceinline__ int wide_slices(const PagedParams& p, const Seq& s, const Division& d) {
-  return ceil_div(seq_tiles(p, s), d.slice);
-}
 
 // Finds wide unit, narrow tile (those of sequences) or token number u.
-template <int BY>
+template <bool WIDE, int BY>
 __device__ __forceinline__ Place find_place(const PagedParams& p, const Division& d, int u, int lane) {
-  auto count = [&](const Seq& s, int& tiles, int& slots) {
-    tiles = slots = 0;
-    if (s.n == 0) return 0;
-    int units = 0;
-    if (is_wide(p, s)) {
-      if (p.wide_units > 0) {
-        const int ns = wide_slices(p, s, d);
-        units = row_groups(p, s.n * p.G) * ns;
-        slots = p.P > 0 || ns > 1 ? units : 0;
-      }
-    } else {
-      tiles = seq_tiles(p, s);
-    }
-    return BY == kWideUnit ? units : BY == kNarrowTile ? tiles : s.n;
-  };
   const int c = (p.B + 63) >> 6;
-  int mine = 0, my_tiles = 0, my_slots = 0;
-  Seq s0{};
-  for (int j = 0; j < c; ++j) {
-    const int b = lane * c + j;
-    if (b >= p.B) break;
-    s0 = load_seq(p, b);
-    int tiles, slots;
-    mine += count(s0, tiles, slots);
-    my_tiles += tiles;
-    my_slots += slots;
-  }
   Place r{};
   r.b = -1;
-  int incl = wave_scan_add(mine);
-  unsigned long long hit = __ballot(u < incl);
-  if (hit == 0) return r;
-  int at = __ffsll(hit) - 1;
-  int base = __builtin_amdgcn_readlane(incl - mine, at);
-  r.tile0 = BY == kNarrowTile ? base : __builtin_amdgcn_readlane(wave_scan_add(my_tiles) - my_tiles, at);
-  r.slot0 = __builtin_amdgcn_readlane(wave_scan_add(my_slots) - my_slots, at);
+  auto hits = [&](const Seq& s, int run_tiles, int run_units) {
+    return __ballot(BY == kToken ? s.n > 0 && u < s.t0 + s.n : u < (BY == kWideUnit ? run_units : run_tiles));
+  };
+  unsigned long long hit = hits(d.s, d.run_tiles, d.run_units);
+  if (hit == 0 && (BY != kToken || c == 1)) return r;
+  Seq s = d.s;
+  int at = hit != 0 ? __ffsll(hit) - 1 : 0;
+  int tile0 = __builtin_amdgcn_readlane(d.run_tiles - d.my_tiles, at);
+  int unit0 = WIDE ? __builtin_amdgcn_readlane(d.run_units - d.my_units, at) : 0;
+  int slot0 = WIDE ? __builtin_amdgcn_readlane(d.run_slots - d.my_slots, at) : 0;
   r.b = at;
-  if (c > 1) {  // lane j looks at the j-th of that lane's sequences (c <= 64: B <= 4096)
-    const int b = at * c + lane;
-    mine = my_tiles = my_slots = 0;
-    if (lane < c && b < p.B) {
-      s0 = load_seq(p, b);
-      mine = count(s0, my_tiles, my_slots);
-    }
-    incl = wave_scan_add(mine);
-    hit = __ballot(u - base < incl);
-    if (hit == 0) {  // (cannot be: the lane's sum exceeds u - base)
+  if (c > 1) {
+    if constexpr (BY == kToken) {  // (a lane's last sequence may be empty: its end is the largest of the lane's)
+      int end = 0;
+      for (int j = 0; j < c && lane * c + j < p.B; ++j) {
+        const Seq x = load_seq(p, lane * c + j);
+        if (x.n > 0) end = x.t0 + x.n;
+      }
+      hit = __ballot(u < end);
       r.b = -1;
-      return r;
+      if (hit == 0) return r;
+      at = __ffsll(hit) - 1;
+      tile0 = __builtin_amdgcn_readlane(d.run_tiles - d.my_tiles, at);
+      if (WIDE) slot0 = __builtin_amdgcn_readlane(d.run_slots - d.my_slots, at);
     }
+    // Lane j looks at the j-th of that lane's sequences (c <= 64: B <= 4096).
     const int first = at * c;
+    int tiles = 0, units = 0, slots = 0;
+    s = Seq{0, 0, 0};
+    if (lane < c && first + lane < p.B) {
+      s = load_seq(p, first + lane);
+      count_seq<WIDE>(p, s, d.slice, tiles, units, slots);
+    }
+    const int rt = wave_scan_add(tiles) + tile0, ru = WIDE ? wave_scan_add(units) + unit0 : 0;
+    const int rs = WIDE ? wave_scan_add(slots) + slot0 : 0;
+    hit = hits(s, rt, ru);
+    r.b = -1;
+    if (hit == 0) return r;
     at = __ffsll(hit) - 1;
     r.b = first + at;
-    base += __builtin_amdgcn_readlane(incl - mine, at);
-    r.tile0 += __builtin_amdgcn_readlane(wave_scan_add(my_tiles) - my_tiles, at);
-    r.slot0 += __builtin_amdgcn_readlane(wave_scan_add(my_slots) - my_slots, at);
+    tile0 = __builtin_amdgcn_readlane(rt - tiles, at);
+    if (WIDE) unit0 = __builtin_amdgcn_readlane(ru - units, at);
+    if (WIDE) slot0 = __builtin_amdgcn_readlane(rs - slots, at);
   }
-  r.s.t0 = __builtin_amdgcn_readlane(s0.t0, at);
-  r.s.n = __builtin_amdgcn_readlane(s0.n, at);
-  r.s.kv = __builtin_amdgcn_readlane(s0.kv, at);
-  r.local = u - base;
+  r.s.t0 = __builtin_amdgcn_readlane(s.t0, at);
+  r.s.n = __builtin_amdgcn_readlane(s.n, at);
+  r.s.kv = __builtin_amdgcn_readlane(s.kv, at);
+  r.tile0 = tile0;
+  r.slot0 = slot0;
+  r.local = u - (BY == kToken ? r.s.t0 : BY == kWideUnit ? unit0 : tile0);
+  if (BY == kToken && r.local < 0) r.b = -1;  // (only where cu_q leaves tokens out)
   return r;
 }
 

@@ -17,7 +17,6 @@
 // before the window, on a page number outside the pool) are zeros in the LDS and masked; rows of a granule that are no
 // keys are replaced by one that is. What memory holds there does not matter.
 #include <climits>
-#include <cstdlib>
 
 #include "common.h"
 
@@ -45,18 +44,8 @@ struct Unit {
   int row0, rows; // first row; rows of the row space (the sequence's, or the whole batch's)
   int lo, hi;     // keys of it that any row of the row group sees
   int k0, k1;     // keys of the unit (k0 a multiple of kTile); those of [lo, hi) count
-  bool whole;     // the unit writes the output; otherwise a partial, to:
-  float* part_o;  // row 0 of its slot
-  float* part_ml;
+  int slot;       // partial slot, or -1: the unit writes the output
 };
-template <int D>
-__device__ __forceinline__ void use_slot(const PagedParams& p, Unit& u, bool wide, int slot, int hk) {
-  const int64_t row = ((int64_t)slot * p.Hkv + hk) * (wide ? p.wide_rows : p.narrow_rows);
-  // (a slot past the last: only where cu_q descends)
-  const bool ok = slot < (wide ? p.wide_slots : p.narrow_slots);
-  u.part_ml = ok ? (wide ? p.wide_ml : p.narrow_ml) + row * 2 : nullptr;
-  u.part_o = (wide ? p.wide_o : p.narrow_o) + row * D;
-}
 // Keys that the rows row0 .. of the sequence see.
 __device__ __forceinline__ void set_range(const PagedParams& p, Unit& u, int most_rows) {
   const int off = u.s.kv - u.s.n;
@@ -69,7 +58,7 @@ __device__ __forceinline__ void set_range(const PagedParams& p, Unit& u, int mos
 // A query row of the unit, as a lane holds it.
 struct Row {
   bool ok;
-  int tok, h;       // token, query head
+  int lse;          // index of the row in lse
   int64_t q, o;     // element offsets of the row in q and o
   int k_lo, k_hi;   // keys it sees: k_lo <= key <= k_hi
 };
@@ -77,13 +66,13 @@ __device__ __forceinline__ Row find_row(const PagedParams& p, const Unit& u, int
   Row x{};
   const int row = u.row0 + rl;
   x.ok = row < u.rows;
-  int i = 0, b = u.b;
+  int i = 0, b = u.b, tok = 0, h = 0;
   Seq s = u.s;
   if (x.ok) {
     i = row / p.G;
-    x.h = hk * p.G + (row - i * p.G);
+    h = hk * p.G + (row - i * p.G);
     if (u.prefix) {
-      x.tok = i;
+      tok = i;
       b = seq_of_token(p, i);
       x.ok = b < p.B;
       if (x.ok) {
@@ -92,12 +81,13 @@ __device__ __forceinline__ Row find_row(const PagedParams& p, const Unit& u, int
         x.ok = i >= 0 && i < s.n;
       }
     } else {
-      x.tok = s.t0 + i;
+      tok = s.t0 + i;
     }
   }
-  if (!x.ok) return Row{false, 0, 0, 0, 0, 0, -1};
-  x.q = (p.cu_q != nullptr ? x.tok * p.q_ss : b * p.q_sb + i * p.q_ss) + x.h * p.q_sh;
-  x.o = (p.cu_q != nullptr ? x.tok * p.o_ss : b * p.o_sb + i * p.o_ss) + x.h * p.o_sh;
+  if (!x.ok) return Row{false, 0, 0, 0, 0, -1};
+  x.q = (p.cu_q != nullptr ? tok * p.q_ss : b * p.q_sb + i * p.q_ss) + h * p.q_sh;
+  x.o = (p.cu_q != nullptr ? tok * p.o_ss : b * p.o_sb + i * p.o_ss) + h * p.o_sh;
+  x.lse = tok * p.Hq + h;
   x.k_hi = min(u.hi, s.kv) - 1;
   x.k_lo = u.lo;
   if (p.causal) x.k_hi = min(x.k_hi, i + s.kv - s.n);
@@ -105,14 +95,29 @@ __device__ __forceinline__ Row find_row(const PagedParams& p, const Unit& u, int
   return x;
 }
 
+__device__ __forceinline__ int64_t shfl64(int64_t x, int lane) {
+  return (int64_t)__shfl((int)(x >> 32), lane, 64) << 32 | (uint32_t)__shfl((int)x, lane, 64);
+}
+
 // What the rows of a wave see together: a block of keys inside [lo_max, hi_min] is seen whole by every row (a row that
 // sees no key makes every block masked; lanes without a row do not count), one outside [lo_min, hi_max] by none.
 struct Seen {
   int lo_max, hi_min, lo_min, hi_max;
 };
-__device__ __forceinline__ Seen seen_by_wave(const Row& x) {
-  const bool empty = x.k_hi < x.k_lo;
+// row: first row of the wave (32 of them).
+__device__ __forceinline__ Seen seen_by_wave(const PagedParams& p, const Unit& u, const Row& x, int row) {
   Seen v;
+  if (!u.prefix) {  // the rows' tokens are i0 .. i1
+    const int off = u.s.kv - u.s.n, last = min(row + 32, u.rows) - 1;
+    const int i0 = row / p.G, i1 = last / p.G;
+    v.lo_min = p.window > 0 ? max(u.lo, i0 + off - p.window + 1) : u.lo;
+    v.lo_max = p.window > 0 ? max(u.lo, i1 + off - p.window + 1) : u.lo;
+    v.hi_min = p.causal ? min(u.hi - 1, i0 + off) : u.hi - 1;
+    v.hi_max = p.causal ? min(u.hi - 1, i1 + off) : u.hi - 1;
+    if (last < row) v = Seen{INT_MAX, INT_MIN, INT_MAX, INT_MIN};  // no row: nothing is full, nothing seen
+    return v;
+  }
+  const bool empty = x.k_hi < x.k_lo;
   v.lo_max = __any(x.ok) ? wave_max_i(!x.ok ? INT_MIN : empty ? INT_MAX : x.k_lo) : INT_MAX;
   v.hi_min = wave_min_i(!x.ok ? INT_MAX : empty ? INT_MIN : x.k_hi);
   v.lo_min = wave_min_i(x.ok && !empty ? x.k_lo : INT_MAX);
@@ -274,9 +279,9 @@ __device__ __forceinline__ void put_state(const State<D>& st, char* slot, f32x2*
 }
 
 // Joins KG states (slot i * step) of a row and writes 8 of its head-dim elements: the output, or a partial of the unit.
-template <typename T, int D, int KG>
+template <typename T, int D, int KG, bool WIDE>
 __device__ __forceinline__ void write_row(const PagedParams& p, const Unit& u, const char* slots, const f32x2* ml, int step,
-                                          int slot_b, int r, int quad, int64_t o_off, int64_t tok_h, int rl, int hk) {
+                                          int slot_b, int r, int quad, int64_t o_off, int lse_at, int rl, int hk) {
   typedef typename T::scalar S;
   typedef typename T::vec8 V8;
   float wt[KG], m = -INFINITY, l = 0.f;
@@ -296,17 +301,19 @@ __device__ __forceinline__ void write_row(const PagedParams& p, const Unit& u, c
     lo += wt[i] * *reinterpret_cast<const f32x4*>(s);
     hi += wt[i] * *reinterpret_cast<const f32x4*>(s + 32 * 16);
   }
-  if (u.whole) {
+  if (u.slot < 0) {
     const float inv = l == 0.f ? 0.f : 1.0f / l;  // a row that sees no key: o = 0, lse = -inf
     st16(static_cast<S*>(p.o) + o_off + 8 * quad,
          from_f32x8<V8>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7) * inv));
-    if (p.lse != nullptr && quad == 0) p.lse[tok_h] = l == 0.f ? -INFINITY : (m + fast_log2(l)) * kLn2;
+    if (p.lse != nullptr && quad == 0) p.lse[lse_at] = l == 0.f ? -INFINITY : (m + fast_log2(l)) * kLn2;
     return;
   }
-  if (u.part_ml == nullptr) return;
-  *reinterpret_cast<f32x4*>(u.part_o + (int64_t)rl * D + 8 * quad) = lo;
-  *reinterpret_cast<f32x4*>(u.part_o + (int64_t)rl * D + 8 * quad + 4) = hi;
-  if (quad == 0) *reinterpret_cast<f32x2*>(u.part_ml + 2 * rl) = f32x2{m, l};
+  if (u.slot >= (WIDE ? p.wide_slots : p.narrow_slots)) return;  // (only where cu_q descends)
+  const int64_t at = ((int64_t)u.slot * p.Hkv + hk) * (WIDE ? p.wide_rows : p.narrow_rows) + rl;
+  float* po = (WIDE ? p.wide_o : p.narrow_o) + at * D + 8 * quad;
+  *reinterpret_cast<f32x4*>(po) = lo;
+  *reinterpret_cast<f32x4*>(po + 4) = hi;
+  if (quad == 0) *reinterpret_cast<f32x2*>((WIDE ? p.wide_ml : p.narrow_ml) + 2 * at) = f32x2{m, l};
 }
 
 // Scores of one 32-key block in the exp2 domain's value units, masked where `masked`; returns their maximum.
@@ -339,29 +346,42 @@ struct Lds {
   static constexpr int WIDE = std::max(2 * 2 * NW * GRAN_B, NW * (SLOT_B + 32 * 8));
 };
 
-// One narrow unit: its keys over NW waves.
-template <typename T, int D, int NW, bool SOFTCAP>
-__device__ __forceinline__ void narrow_unit(const Unit& u, char* smem, int hk) {
-  typedef DmaLayout<D> L;
+// A wave's tiles of a narrow unit: every NW-th of the 32-key tiles that hold a key.
+template <int NW>
+struct NarrowTiles {
+  int lane, w, t_first, n;
+  __device__ __forceinline__ explicit NarrowTiles(const Unit& u) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // the lane constants are made anew for each unit: kept over all of them, they spill
+    lane = tid & 63;
+    w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    t_first = max(u.k0, u.lo) / 32;
+    n = u.k1 > u.k0 ? max(0, (ceil_div(min(u.k1, u.hi), 32) - t_first - w + NW - 1) / NW) : 0;
+  }
+  __device__ __forceinline__ int tile(int s) const { return t_first + w + NW * s; }
+  // The lanes' granules of 32 tiles from the wave's tile s on.
+  __device__ __forceinline__ int granule(int s) const { return 2 * tile(s + (lane >> 1)) + (lane & 1); }
+  __device__ __forceinline__ int first_page(const PagedParams& p, const Unit& u) const {
+    Granules gr;
+    gr.row = p.table + u.b * p.table_sb;
+    return n > 0 ? gr.page_of(p, granule(0)) : 0;
+  }
+};
+
+// One narrow unit: its keys over NW waves. page: first_page(); ahead(): called when the first copies are on their way.
+template <typename T, int D, int NW, bool SOFTCAP, typename F>
+__device__ __forceinline__ void narrow_unit(const Unit& u, char* smem, int hk, int page, F&& ahead) {
   typedef typename T::scalar S;
   typedef typename T::vec8 V8;
   typedef typename T::vec4 V4;
   constexpr int TILE_B = Lds<D, NW>::TILE_B, GRAN_B = Lds<D, NW>::GRAN_B, WAVE_B = Lds<D, NW>::WAVE_B;
   constexpr int LOADS = 2 * GranuleCopy<D, true>::LOADS;   // direct loads of a tile, K or V
   const PagedParams& p = fresh_params();
-  int tid = threadIdx.x;
-  asm volatile("" : "+v"(tid));  // the lane constants are made anew for each unit: kept over all of them, they spill
-  const int lane = tid & 63, r = lane & 31, g = lane >> 5;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-
-  // The wave's tiles: every NW-th of the slice's 32-key tiles that hold a key.
-  const int t_first = max(u.k0, u.lo) / 32, t_end = ceil_div(min(u.k1, u.hi), 32);
-  const int n_own = u.k1 > u.k0 ? max(0, ceil_div(t_end - t_first - w, NW)) : 0;
-  auto tile_of = [&](int s) { return t_first + w + NW * s; };
-  auto gran_of = [&](int s0) { return 2 * tile_of(s0 + (lane >> 1)) + (lane & 1); };
+  const NarrowTiles<NW> mine(u);
+  const int lane = mine.lane, w = mine.w, tid = 64 * w + lane, r = lane & 31, g = lane >> 5, n_own = mine.n;
   Granules gr;
   gr.row = p.table + u.b * p.table_sb;
-  if (n_own > 0) gr.next = gr.page_of(p, gran_of(0));
+  gr.next = page;
 
   const Row x = find_row(p, u, r, hk);
   const S* qp = static_cast<const S*>(p.q) + x.q;
@@ -385,7 +405,7 @@ __device__ __forceinline__ void narrow_unit(const Unit& u, char* smem, int hk) {
     const int64_t ss_b = values ? v_ss_b : k_ss_b;
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
-      const int at = 2 * (s & 31) + hh, key = tile_of(s) * 32 + hh * kGranule;
+      const int at = 2 * (s & 31) + hh, key = mine.tile(s) * 32 + hh * kGranule;
       const uint32_t lds = wave_at + (values ? TILE_B : 0) + hh * GRAN_B;
       const char* base = values ? vp + gr.offset(p, key / kGranule, at, p.v_sp, p.v_ss)
                                 : kp + gr.offset(p, key / kGranule, at, p.k_sp, p.k_ss);
@@ -397,24 +417,25 @@ __device__ __forceinline__ void narrow_unit(const Unit& u, char* smem, int hk) {
   };
   auto holes_of = [&](int s) { return ~(unsigned)(gr.live >> (2 * (s & 31))) & 3u; };
 
-  const Seen see = seen_by_wave(x);
+  const Seen see = seen_by_wave(p, u, x, u.row0);
   State<D> st;
   st.init();
   const float c = score_coeff<SOFTCAP, 0>(p.s);
   unsigned holes = 0;
   if (n_own > 0) {
-    gr.take(p, u, gran_of(0), gran_of(32));
+    gr.take(p, u, mine.granule(0), mine.granule(32));
     copy(0, false);
     copy(0, true);
     holes = holes_of(0);
   }
+  ahead();
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk) {
     asm volatile("" : "+v"(qf[kk]));
     if (!x.ok) qf[kk] = V8{};
   }
   for (int s = 0; s < n_own; ++s) {
-    const int kt = tile_of(s) * 32;
+    const int kt = mine.tile(s) * 32;
     const bool more = s + 1 < n_own;
     const bool live = holes != 3 && kt <= see.hi_max && kt + 31 >= see.lo_min;
     const bool full = holes == 0 && kt >= see.lo_max && kt + 31 <= see.hi_min;
@@ -432,7 +453,7 @@ __device__ __forceinline__ void narrow_unit(const Unit& u, char* smem, int hk) {
     // before its offsets are given up: V of tile s + 1 below uses the window that K took up.)
     unsigned next_holes = 0;
     if (more) {
-      if (((s + 1) & 31) == 0) gr.take(p, u, gran_of(s + 1), gran_of(s + 33));
+      if (((s + 1) & 31) == 0) gr.take(p, u, mine.granule(s + 1), mine.granule(s + 33));
       next_holes = holes_of(s + 1);
       copy(s + 1, false);
     }
@@ -476,64 +497,75 @@ __device__ __forceinline__ void narrow_unit(const Unit& u, char* smem, int hk) {
   put_state(st, slots + w * WAVE_B, ml + 32 * w, c, lane);
   __syncthreads();
   const PagedParams& pe = fresh_params();
-  const int live_rows = min(32, u.rows - u.row0);
-  for (int it = tid; it < live_rows * (D / 8); it += 64 * NW) {
-    const int row = it / (D / 8), quad = it % (D / 8);
-    const Row y = find_row(pe, u, row, hk);
-    if (!y.ok) continue;
-    write_row<T, D, NW>(pe, u, slots, ml, 1, WAVE_B, row, quad, y.o, (int64_t)y.tok * pe.Hq + y.h, row, hk);
+  const int items = min(32, u.rows - u.row0) * (D / 8);
+  for (int it0 = 0; it0 < items; it0 += 64 * NW) {
+    const int it = it0 + tid, row = min(it / (D / 8), 31), quad = it % (D / 8);
+    const int64_t o_off = shfl64(x.o, row);  // (the lane that holds the row, in every wave)
+    const int lse_at = __shfl(x.lse, row, 64);
+    const bool ok = __shfl((int)x.ok, row, 64);
+    if (it < items && ok) write_row<T, D, NW, false>(pe, u, slots, ml, 1, WAVE_B, row, quad, o_off, lse_at, row, hk);
   }
 }
 
-// The stretch of narrow workgroup `wg`, segment by segment.
-template <typename T, int D, int NW, bool SOFTCAP>
+// Segment of the stretch that begins with tile f and ends before `to`; returns where it ends (0: there is none).
+template <bool WIDE>
+__device__ __forceinline__ int narrow_segment(const PagedParams& p, const Division& d, int f, int to, int wg, Unit& u) {
+  u.row0 = 0;
+  int first, tiles, index;  // the segment's sequence: its first tile and their number, and its place in the slots
+  if (f < d.p_tiles) {
+    u.prefix = true;
+    u.b = 0;
+    u.s = Seq{0, 0, 0};
+    u.rows = p.T * p.G;
+    u.lo = d.p_lo;
+    u.hi = p.P;
+    first = index = 0;
+    tiles = d.p_tiles;
+  } else {
+    const Place pl = find_place<WIDE, kNarrowTile>(p, d, f - d.p_tiles, threadIdx.x & 63);
+    if (pl.b < 0) return 0;
+    u.prefix = false;
+    u.b = pl.b;
+    u.s = pl.s;
+    u.rows = pl.s.n * p.G;
+    u.lo = first_key(p, u.s);
+    u.hi = pl.s.kv;
+    first = d.p_tiles + pl.tile0;
+    index = pl.b + (d.p_tiles > 0 ? 1 : 0);
+    tiles = seq_tiles(p, u.s);
+  }
+  const int last = min(to, first + tiles), t0 = u.lo / kTile;
+  u.k0 = (t0 + f - first) * kTile;
+  u.k1 = (t0 + last - first) * kTile;
+  u.slot = p.P == 0 && f == first && last == first + tiles ? -1 : wg + index;
+  return last;
+}
+
+// The stretch of narrow workgroup `wg`, segment by segment. The first page numbers of the next segment are requested while
+// the present one streams: behind its 32 MB in flight a load takes 5 us.
+template <typename T, int D, int NW, bool WIDE, bool SOFTCAP>
 __device__ __forceinline__ void narrow_stretch(const Division& d, char* smem, int hk, int wg) {
   const int from = wg * d.stretch, to = min(d.tiles, from + d.stretch);
+  int page = 0;
   for (int f = from; f < to;) {
-    const PagedParams& p = fresh_params();
     Unit u;
-    u.row0 = 0;
-    int first, tiles, index;  // the segment's sequence: its first tile and their number, and its place in the slots
-    if (f < d.p_tiles) {
-      u.prefix = true;
-      u.b = 0;
-      u.s = Seq{0, 0, 0};
-      u.rows = p.T * p.G;
-      u.lo = d.p_lo;
-      u.hi = p.P;
-      first = index = 0;
-      tiles = d.p_tiles;
-    } else {
-      int lane = threadIdx.x & 63;
-      asm volatile("" : "+v"(lane));
-      const Place pl = find_place<kNarrowTile>(p, d, f - d.p_tiles, lane);
-      if (pl.b < 0) return;
-      u.prefix = false;
-      u.b = pl.b;
-      u.s = pl.s;
-      u.rows = pl.s.n * p.G;
-      first = d.p_tiles + pl.tile0;
-      index = pl.b + (d.p_tiles > 0 ? 1 : 0);
-      set_range(p, u, kNarrowRows);
-      u.lo = first_key(p, u.s);
-      tiles = seq_tiles(p, u.s);
-    }
-    const int last = min(to, first + tiles);
-    const int t0 = u.lo / kTile;
-    u.k0 = (t0 + f - first) * kTile;
-    u.k1 = (t0 + last - first) * kTile;
-    u.whole = p.P == 0 && f == first && last == first + tiles;
-    use_slot<D>(p, u, false, wg + index, hk);
-    narrow_unit<T, D, NW, SOFTCAP>(u, smem, hk);
-    f = last;
+    const int next = narrow_segment<WIDE>(fresh_params(), d, f, to, wg, u);
+    if (next == 0) return;
+    if (f == from) page = NarrowTiles<NW>(u).first_page(fresh_params(), u);
+    narrow_unit<T, D, NW, SOFTCAP>(u, smem, hk, page, [&]() __attribute__((always_inline)) {
+      if (next >= to) return;
+      Unit v;
+      if (narrow_segment<WIDE>(fresh_params(), d, next, to, wg, v) != 0)
+        page = NarrowTiles<NW>(v).first_page(fresh_params(), v);
+    });
+    f = next;
     if (f < to) __syncthreads();  // the states in the LDS are read
   }
 }
 
-template <int D>
-__device__ __forceinline__ bool wide_unit_of(const PagedParams& p, const Division& d, int n, int hk, Unit& u) {
+__device__ __forceinline__ bool wide_unit_of(const PagedParams& p, const Division& d, int n, Unit& u) {
   const int R = 1 << p.log2_r, p_units = d.p_rg * d.p_ns;
-  int k, ns, slot;
+  int k, ns;
   u.prefix = n < p_units;
   if (u.prefix) {
     k = n / d.p_rg;
@@ -543,26 +575,23 @@ __device__ __forceinline__ bool wide_unit_of(const PagedParams& p, const Divisio
     u.s = Seq{0, 0, 0};
     u.row0 = rg * R;
     u.rows = p.T * p.G;
-    slot = rg * d.p_ns + k;
+    u.slot = rg * d.p_ns + k;
     u.lo = d.p_lo;
     u.hi = p.P;
-    u.whole = false;
   } else {
-    const Place pl = find_place<kWideUnit>(p, d, n - p_units, threadIdx.x & 63);
+    const Place pl = find_place<true, kWideUnit>(p, d, n - p_units, threadIdx.x & 63);
     if (pl.b < 0) return false;
     const int nrg = row_groups(p, pl.s.n * p.G);
-    ns = wide_slices(p, pl.s, d);
+    ns = wide_slices(p, pl.s, d.slice);
     k = pl.local / nrg;
     const int rg = pl.local - k * nrg;
     u.b = pl.b;
     u.s = pl.s;
     u.row0 = rg * R;
     u.rows = pl.s.n * p.G;
-    slot = p_units + pl.slot0 + rg * ns + k;
-    u.whole = p.P == 0 && ns == 1;
+    u.slot = p.P == 0 && ns == 1 ? -1 : p_units + pl.slot0 + rg * ns + k;
     set_range(p, u, R);
   }
-  use_slot<D>(p, u, true, slot, hk);
   const int tiles = key_tiles(u.lo, u.hi), per = ceil_div(tiles, ns), t0 = u.lo / kTile;
   u.k0 = (t0 + min(tiles, k * per)) * kTile;
   u.k1 = (t0 + min(tiles, (k + 1) * per)) * kTile;
@@ -647,7 +676,7 @@ __device__ __forceinline__ void wide_unit(const Unit& u, char* smem, int hk) {
     }
   };
 
-  const Seen see = seen_by_wave(x);
+  const Seen see = seen_by_wave(p, u, x, u.row0 + 32 * wr);
   State<D> st;
   st.init();
   const float c = score_coeff<SOFTCAP, 0>(p.s);
@@ -746,6 +775,7 @@ __device__ __forceinline__ void wide_unit(const Unit& u, char* smem, int hk) {
         const V4 a1 = tr_read_at(vbase[fr.vb(db, 1)] + fr.vo(kk, 1), S{});
         st.o[db] = mfma32(__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7), pb, st.o[db]);
       }
+      asm volatile("" : "+v"(st.l[0]), "+v"(st.l[1]));  // (the sums stay among the MFMAs)
     }
   };
 
@@ -785,27 +815,31 @@ __device__ __forceinline__ void wide_unit(const Unit& u, char* smem, int hk) {
   put_state(st, smem + w * SLOT_B, ml + 32 * w, c, lane);
   __syncthreads();
   const PagedParams& pe = fresh_params();
-  const int live_rows = min(32 * NWR, u.rows - u.row0);
-  for (int it = tid; it < live_rows * (D / 8); it += 64 * NW) {
-    const int row = it / (D / 8), quad = it % (D / 8);
-    const Row y = find_row(pe, u, row, hk);
-    if (!y.ok) continue;
-    write_row<T, D, KG>(pe, u, smem + (row / 32) * SLOT_B, ml + 32 * (row / 32), NWR, SLOT_B, row % 32, quad, y.o,
-                        (int64_t)y.tok * pe.Hq + y.h, row, hk);
+  // Each wave writes a KG-th of the rows that it holds.
+  constexpr int RW = 32 / KG;
+#pragma unroll 2
+  for (int it = lane; it < RW * (D / 8); it += 64) {
+    const int row = kg * RW + it / (D / 8), quad = it % (D / 8);
+    const int64_t o_off = shfl64(x.o, row);
+    const int lse_at = __shfl(x.lse, row, 64);
+    const bool ok = __shfl((int)x.ok, row, 64);
+    if (ok)
+      write_row<T, D, KG, true>(pe, u, smem + wr * SLOT_B, ml + 32 * wr, NWR, SLOT_B, row, quad, o_off, lse_at,
+                                32 * wr + row, hk);
   }
 }
 
 constexpr int kNarrowWaves = 4;
 
-// Everything narrow. Waves per SIMD: as many workgroups per CU as the LDS holds (33 KiB at head_dim 64, 67 at 128, 133 at
-// 256).
+// Everything narrow. Waves per SIMD: as many workgroups per CU as the LDS holds (67 KiB at head_dim 128, 133 at 256);
+// three at 64.
 template <typename T, int D, bool SOFTCAP>
 __global__ void __launch_bounds__(64 * kNarrowWaves)
-__attribute__((amdgpu_waves_per_eu(D >= 256 ? 1 : D >= 128 ? 2 : 4))) paged_narrow_kernel(PagedParams p) {
+__attribute__((amdgpu_waves_per_eu(D >= 256 ? 1 : D >= 128 ? 2 : 3))) paged_narrow_kernel(PagedParams p) {
   __shared__ __attribute__((aligned(1024))) char smem[Lds<D, kNarrowWaves>::NARROW];
   const int hk = blockIdx.x % p.Hkv, n = blockIdx.x / p.Hkv;
-  const Division d = divide(p, threadIdx.x & 63);
-  narrow_stretch<T, D, kNarrowWaves, SOFTCAP>(d, smem, hk, n);
+  const Division d = divide<false>(p, threadIdx.x & 63);
+  narrow_stretch<T, D, kNarrowWaves, false, SOFTCAP>(d, smem, hk, n);
 }
 
 // Narrow stretches, then wide units.
@@ -814,13 +848,13 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OC
 paged_mixed_kernel(PagedParams p) {
   __shared__ __attribute__((aligned(1024))) char smem[std::max(Lds<D, NW>::NARROW, Lds<D, NW>::WIDE)];
   const int hk = blockIdx.x % p.Hkv, n = blockIdx.x / p.Hkv;
-  const Division d = divide(p, threadIdx.x & 63);
+  const Division d = divide<true>(p, threadIdx.x & 63);
   if (n < p.narrow_wgs) {
-    narrow_stretch<T, D, NW, SOFTCAP>(d, smem, hk, n);
+    narrow_stretch<T, D, NW, true, SOFTCAP>(d, smem, hk, n);
     return;
   }
   Unit u;
-  if (wide_unit_of<D>(p, d, n - p.narrow_wgs, hk, u)) wide_unit<T, D, NW, KG, OCC, SOFTCAP>(u, smem, hk);
+  if (wide_unit_of(p, d, n - p.narrow_wgs, u)) wide_unit<T, D, NW, KG, OCC, SOFTCAP>(u, smem, hk);
 }
 
 // Joins the partials of rows: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, lse = (M + log2 L) ln 2, with those of the
@@ -828,7 +862,7 @@ paged_mixed_kernel(PagedParams p) {
 // numbers them) of a KV head. Its groups of D / 4 threads (four head-dim elements each) take rows, or, where a row has many
 // partials, share one.
 constexpr int kMergeThreads = 256;
-template <typename T, int D>
+template <typename T, int D, bool WIDE>
 __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(PagedParams p) {
   typedef typename T::scalar S;
   typedef typename T::vec4 V4;
@@ -838,18 +872,18 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(PagedParams 
   const int tid = threadIdx.x, lane = tid & 63, col = tid % COLS, grp = tid / COLS;
   const int hk = blockIdx.x % p.Hkv;
   const int from = blockIdx.x / p.Hkv * p.rows_per_merge, to = min(p.T * p.G, from + p.rows_per_merge);
-  const Division d = divide(p, lane);
+  const Division d = divide<WIDE>(p, lane);
   for (int f = from; f < to;) {
-    const Place pl = find_place<kToken>(p, d, f / p.G, lane);
+    const Place pl = find_place<WIDE, kToken>(p, d, f / p.G, lane);
     if (pl.b < 0) return;  // behind the last sequence
     const int r_from = pl.local * p.G + (f - f / p.G * p.G);  // rows of the sequence
     const int r_to = min(pl.s.n * p.G, r_from + (to - f));
     f += r_to - r_from;
     // Its own partials: slots own0 + (wide: row group * ns) + 0 .. n_own - 1; the prefix's likewise.
-    const bool wide = is_wide(p, pl.s);
+    const bool wide = WIDE && is_wide(p, pl.s);
     int n_own, own0;
     if (wide) {
-      n_own = wide_slices(p, pl.s, d);
+      n_own = wide_slices(p, pl.s, d.slice);
       own0 = d.p_rg * d.p_ns + pl.slot0;
     } else {
       const int t0 = d.p_tiles + pl.tile0, t1 = t0 + seq_tiles(p, pl.s) - 1;
@@ -884,7 +918,8 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(PagedParams 
       };
       const int rg = rc >> p.log2_r, prg = prow >> p.log2_r, rmask = (1 << p.log2_r) - 1;
       locate(wide, own0 + (wide ? rg * n_own : 0), wide ? rc & rmask : rc, own_o, own_ml, own_step);
-      locate(p.prefix_wide, p.prefix_wide ? prg * d.p_ns : 0, p.prefix_wide ? prow & rmask : prow, pre_o, pre_ml, pre_step);
+      const bool pw = WIDE && p.prefix_wide;
+      locate(pw, pw ? prg * d.p_ns : 0, pw ? prow & rmask : prow, pre_o, pre_ml, pre_step);
       float M = -INFINITY, Ls = 0.f;
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
       constexpr int U = 4;  // partials in flight
@@ -954,20 +989,31 @@ struct HostPlan {
     return ((int64_t)wide_slots * wide_rows + (int64_t)narrow_slots * narrow_rows) * Hkv * (D + 2);
   }
 };
-int env(const char* n, int d) { return getenv(n) ? atoi(getenv(n)) : d; }
+// Row groups. 64 rows (waves in pairs over the same rows) where there are no more; otherwise 128 rows, two workgroups of
+// four waves per CU, so that one streams or computes while the other begins or ends; but at head_dim 128 256 rows, one
+// workgroup of eight waves, for chunks that fill the chip with them: half the keys and values through the LDS. Measured on
+// MI355X, bf16, 32 / 8 heads, 128 / 256 rows, us: 2 x 1,024 tokens, 8,192 keys 272 / 245; 16 x 128, 2,048 92 / 83; 8 x 512,
+// 512 55 / 52; 4 x 128, 4,096 57.5 / 57.7; 262 tokens of 16 sequences behind a prefix of 16,384 104 / 122; a step of 28
+// decode rows and 4 chunks 137 / 146.
+// Units wanted: as many as are resident at once or a little fewer, for the row groups' last slices are short (the same
+// step at 256, 384, 448, 512 units 138, 136, 135, 131; 8 chunks of up to 1,024 tokens 148, 147, 147, 158; the prefix of
+// 16,384 133, 106, 101, 100).
+// Narrow stretches: one for each resident workgroup, of at most two per CU (32 x 16 heads of 64, up to 4,000 keys: 512
+// stretches 53, 768 56); beside wide units three quarters of them, so that both begin at once
+// (the step at 256, 384, 512 stretches 138, 137, 157).
 HostPlan host_plan(int64_t B, int64_t T, bool ragged, int64_t Hq, int64_t Hkv, int64_t D, int64_t P) {
   HostPlan h{};
-  const int64_t G = Hq / Hkv, Sq = T / B;
+  const int64_t G = Hq / Hkv, Sq = T / B, CUs = 256;
   const int64_t most = (ragged ? T : Sq) * G;  // most rows that a sequence can have
   h.prefix_wide = P > 0 && T * G > dgg_paged::kNarrowRows;
   const bool wide = most > dgg_paged::kNarrowRows || h.prefix_wide;
-  const bool narrow = ragged || Sq * G <= dgg_paged::kNarrowRows || (P > 0 && !h.prefix_wide);
+  const bool narrow = ragged || most <= dgg_paged::kNarrowRows;
+  const int64_t per_cu = D == 64 ? 3 : D == 128 ? 2 : 1;  // workgroups of four waves on a CU
   if (wide) {
-    // Rows that a wide unit finds: those of the prefix, or of the average sequence that is wide, if half of them are.
     const int64_t typical = h.prefix_wide ? T * G : ragged ? 2 * T * G / B : most;
-    const int widest = D == 128 ? 8 : 7;
-    h.log2_r = env("DGG_R", typical <= 64 ? 6 : typical <= 128 || widest == 7 ? 7 : 8);
-    h.wide_target = std::max<int>(1, env("DGG_T", 256) / Hkv);
+    const bool large = D == 128 && !ragged && T * G / 256 * Hkv >= CUs;
+    h.log2_r = typical <= 64 ? 6 : large ? 8 : 7;
+    h.wide_target = (int)std::max<int64_t>(1, (large ? CUs : CUs * per_cu * 7 / 8) / Hkv);
     const int64_t R = 1ll << h.log2_r;
     // ragged: a sequence's rows fill row groups but for its last; only sequences of more than 32 rows count
     const int64_t nrg = ragged ? T * G / R + std::min(B, T * G / (dgg_paged::kNarrowRows + 1))
@@ -978,7 +1024,7 @@ HostPlan host_plan(int64_t B, int64_t T, bool ragged, int64_t Hq, int64_t Hkv, i
     h.wide_rows = (int)std::min<int64_t>(R, h.prefix_wide ? T * G : most);
   }
   if (narrow) {
-    h.narrow_wgs = std::max<int>(1, env("DGG_N", wide ? 256 : 512) / Hkv);
+    h.narrow_wgs = (int)std::max<int64_t>(1, (wide ? CUs * per_cu * 3 / 4 : CUs * std::min<int64_t>(per_cu, 2)) / Hkv);
     h.narrow_slots = (int)(h.narrow_wgs + B + 1);
     h.narrow_rows = (int)std::min<int64_t>(dgg_paged::kNarrowRows, P > 0 && !h.prefix_wide ? T * G : most);
   }
@@ -990,12 +1036,14 @@ void launch_cap(const PagedParams& p, hipStream_t st) {
   const dim3 grid((unsigned)(p.wide_units + p.narrow_wgs) * p.Hkv);
   if (p.wide_units == 0)
     hipLaunchKernelGGL((paged_narrow_kernel<T, D, SOFTCAP>), grid, dim3(64 * kNarrowWaves), 0, st, p);
-  else if constexpr (D == 128) {
-    if (p.log2_r == 6) hipLaunchKernelGGL((paged_mixed_kernel<T, D, 8, 4, 2, SOFTCAP>), grid, dim3(512), 0, st, p);
-    else if (p.log2_r == 7) hipLaunchKernelGGL((paged_mixed_kernel<T, D, 8, 2, 2, SOFTCAP>), grid, dim3(512), 0, st, p);
-    else hipLaunchKernelGGL((paged_mixed_kernel<T, D, 8, 1, 2, SOFTCAP>), grid, dim3(512), 0, st, p);
-  } else {
-    constexpr int OCC = D == 64 ? 3 : 1;
+  else {
+    constexpr int OCC = D == 64 ? 3 : D == 128 ? 2 : 1;
+    if constexpr (D == 128) {
+      if (p.log2_r == 8) {
+        hipLaunchKernelGGL((paged_mixed_kernel<T, D, 8, 1, OCC, SOFTCAP>), grid, dim3(512), 0, st, p);
+        return;
+      }
+    }
     if (p.log2_r == 6) hipLaunchKernelGGL((paged_mixed_kernel<T, D, 4, 2, OCC, SOFTCAP>), grid, dim3(256), 0, st, p);
     else hipLaunchKernelGGL((paged_mixed_kernel<T, D, 4, 1, OCC, SOFTCAP>), grid, dim3(256), 0, st, p);
   }
@@ -1006,7 +1054,10 @@ void launch(const PagedParams& p, hipStream_t st) {
   else launch_cap<T, D, false>(p, st);
   const int64_t rows = (int64_t)p.T * p.G;
   const int64_t wgs = (rows + p.rows_per_merge - 1) / p.rows_per_merge * p.Hkv;
-  hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3((unsigned)wgs), dim3(kMergeThreads), 0, st, p);
+  if (p.wide_units > 0)
+    hipLaunchKernelGGL((paged_merge_kernel<T, D, true>), dim3((unsigned)wgs), dim3(kMergeThreads), 0, st, p);
+  else
+    hipLaunchKernelGGL((paged_merge_kernel<T, D, false>), dim3((unsigned)wgs), dim3(kMergeThreads), 0, st, p);
 }
 
 int check_sizes(const char* op, int64_t B, int64_t T, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix) {
