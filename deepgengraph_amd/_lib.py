@@ -79,9 +79,9 @@ SIGNATURES = {
     "dgg_attn_splitkv_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),
     "dgg_attn_splitkv": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64p, _i64,
                                 _f32, _f32, _i64, _u32, _i32, _vp]),
-    "dgg_paged_append": (_i32, [_vp] * 9 + [_i64] * 9 + [_i64p, _f32, _i32, _vp]),
+    "dgg_paged_append": (_i32, [_vp] * 9 + [_i64] * 9 + [_vp, _f32, _i32, _vp]),
     "dgg_attn_paged_workspace_bytes": (_i64, [_i64] * 7),
-    "dgg_attn_paged": (_i32, [_vp] * 9 + [_i64] * 11 + [_i64p, _f32, _f32, _i64, _u32, _i32, _vp]),
+    "dgg_attn_paged": (_i32, [_vp] * 9 + [_i64] * 11 + [_vp, _f32, _f32, _i64, _u32, _i32, _vp]),
     "dgg_attn_decode": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64p, _i64, _f32,
                                _i32, _vp]),
 }

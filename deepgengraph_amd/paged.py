@@ -15,45 +15,71 @@ cache of one length for all sequences (deepgengraph_exp/cases/kernels/attn.py:18
 """
 from __future__ import annotations
 
+import functools
 import math
+import struct
 
 import torch
 
 from . import _lib
-from .attention import _check_bshd
+
+_I32 = torch.int32
+_STRIDES_19, _STRIDES_13 = struct.Struct("19q"), struct.Struct("13q")
 
 
-def _tokens(name: str, t: torch.Tensor, cu_q):
-    """(B, T, Sq, [batch, token, head] strides) of a step's tokens; Sq 0 with cu_q."""
+# A step's small calls take the GPU 5 to 15 us, and the host about as long: the checks below look at each property once,
+# in the cheapest form, and leave what the library checks itself (sizes, strides, alignment) to it.
+def _device(*tensors):
+    """The common GPU's index; None stands for an argument that was not given."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index or index < 0:
+            _lib.require_gpu(*tensors)  # says what is wrong
+    return index
+
+
+def _tokens(op: str, name: str, t: torch.Tensor, cu_q):
+    """(batch, token, head) strides of a step's tokens."""
     st = t.stride()
-    if t.dim() != (4 if cu_q is None else 3):
-        raise RuntimeError(f"{name}: expected {'[B, Sq, heads, D]' if cu_q is None else '[T, heads, D] with cu_q'}, got "
-                           f"shape {tuple(t.shape)}")
+    if len(st) != (4 if cu_q is None else 3):
+        raise RuntimeError(f"{op}: {name} must be {'[B, Sq, heads, D]' if cu_q is None else '[T, heads, D] with cu_q'}, "
+                           f"got shape {tuple(t.shape)}")
     if st[-1] != 1:
-        raise RuntimeError(f"{name}: head dimension must be contiguous (stride {st[-1]})")
-    if cu_q is None:
-        return t.shape[0], t.shape[0] * t.shape[1], t.shape[1], st[:3]
-    return cu_q.shape[0] - 1, t.shape[0], 0, (0, st[0], st[1])
+        raise RuntimeError(f"{op}: {name}'s head dimension must be contiguous (stride {st[-1]})")
+    return st[:3] if cu_q is None else (0, st[0], st[1])
 
 
 def _cache(op: str, k_pages, v_pages, block_table, kv_lens, cu_q, B: int):
-    """Checks of the pools, the table and the lengths."""
-    _check_bshd("k_pages", k_pages)
-    _check_bshd("v_pages", v_pages)
-    if v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
-        raise RuntimeError(f"{op}: k_pages {tuple(k_pages.shape)} {k_pages.dtype} and v_pages {tuple(v_pages.shape)} "
-                           f"{v_pages.dtype} differ")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or (
-            block_table.shape[1] > 1 and block_table.stride(1) != 1):
+    """Checks of the pools, the table and the lengths; (shape of the pools, table width, strides of both pools)."""
+    shape, ks, vs = k_pages.shape, k_pages.stride(), v_pages.stride()
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype is not k_pages.dtype:
+        raise RuntimeError(f"{op}: k_pages {tuple(shape)} {k_pages.dtype} and v_pages {tuple(v_pages.shape)} "
+                           f"{v_pages.dtype} must be two [pages, page_size, Hkv, D] of one kind")
+    if ks[3] != 1 or vs[3] != 1:
+        raise RuntimeError(f"{op}: the pages' head dimension must be contiguous (strides {ks[3]}, {vs[3]})")
+    table = block_table.shape
+    if block_table.dtype is not _I32 or len(table) != 2 or table[0] != B or (table[1] > 1 and block_table.stride(1) != 1):
         raise RuntimeError(f"{op}: block_table must be int32 [{B}, width] with unit column stride")
-    if kv_lens.dtype != torch.int32 or kv_lens.shape != (B,) or not kv_lens.is_contiguous():
+    if kv_lens.dtype is not _I32 or kv_lens.shape != (B,) or not kv_lens.is_contiguous():
         raise RuntimeError(f"{op}: kv_lens must be contiguous int32 [{B}]")
+    return shape, table[1], ks[:3] + vs[:3]
 
 
-def _check_cu(op: str, cu_q):
-    if cu_q is not None and (cu_q.dtype != torch.int32 or cu_q.dim() != 1 or cu_q.shape[0] < 1
-                             or not cu_q.is_contiguous()):
+def _batch(op: str, t: torch.Tensor, cu_q):
+    """(B, T, Sq) of a step's tokens; Sq 0 with cu_q."""
+    if cu_q is None:
+        return t.shape[0], t.shape[0] * t.shape[1], t.shape[1]
+    if cu_q.dtype is not _I32 or cu_q.dim() != 1 or cu_q.shape[0] < 1 or not cu_q.is_contiguous():
         raise RuntimeError(f"{op}: cu_q must be contiguous int32 [B + 1]")
+    return cu_q.shape[0] - 1, t.shape[0], 0
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(op: str, *sizes: int) -> int:
+    need = _lib.load().dgg_attn_paged_workspace_bytes(*sizes)
+    if need < 0:
+        raise RuntimeError(f"{op}: {_lib.load().dgg_last_error().decode(errors='replace')}")
+    return need
 
 
 def paged_append(key: torch.Tensor, value: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -72,70 +98,64 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, k_pages: torch.Tensor, 
     cu_q[B] on are not touched. Two tokens of one call must not share a place: a page that two sequences share is
     written by neither."""
     op = "paged_append"
-    dev = _lib.require_gpu(key, value, k_pages, v_pages, block_table, kv_lens, query, cu_q, query_out)
-    _check_cu(op, cu_q)
-    B, T, Sq, k_st = _tokens("key", key, cu_q)
-    _, _, _, v_st = _tokens("value", value, cu_q)
-    _cache(op, k_pages, v_pages, block_table, kv_lens, cu_q, B)
-    n_pages, page, Hkv, D = k_pages.shape
-    if value.shape != key.shape or tuple(key.shape[-2:]) != (Hkv, D):
-        raise RuntimeError(f"{op}: key {tuple(key.shape)} and value {tuple(value.shape)} do not match pages of "
-                           f"{Hkv} heads of {D}")
-    if not (key.dtype == value.dtype == k_pages.dtype):
+    dev = _device(key, value, k_pages, v_pages, block_table, kv_lens, query, cu_q, query_out)
+    k_st, v_st = _tokens(op, "key", key, cu_q), _tokens(op, "value", value, cu_q)
+    B, T, Sq = _batch(op, key, cu_q)
+    (n_pages, page, Hkv, D), width, pool_st = _cache(op, k_pages, v_pages, block_table, kv_lens, cu_q, B)
+    shape, dtype = key.shape, key.dtype
+    if value.shape != shape or shape[-2] != Hkv or shape[-1] != D:
+        raise RuntimeError(f"{op}: key {tuple(shape)} and value {tuple(value.shape)} do not match pages of {Hkv} heads "
+                           f"of {D}")
+    if value.dtype is not dtype or k_pages.dtype is not dtype:
         raise RuntimeError(f"{op}: key, value and page dtypes differ")
-    Hq, q_st, o_st = 0, (0, 0, 0), (0, 0, 0)
+    if rope_theta is not None and not rope_theta > 0:
+        raise RuntimeError(f"{op}: rope_theta must be > 0 (got {rope_theta})")
+    Hq, q_st, o_st, q_ptr, o_ptr = 0, (0, 0, 0), (0, 0, 0), None, None
     if query is not None:
         if rope_theta is None:
             raise RuntimeError(f"{op}: a query is taken to be rotated: give rope_theta")
-        _, _, _, q_st = _tokens("query", query, cu_q)
-        if query.shape[:-2] != key.shape[:-2] or query.shape[-1] != D or query.dtype != key.dtype:
-            raise RuntimeError(f"{op}: query {tuple(query.shape)} {query.dtype} does not match key {tuple(key.shape)}")
+        q_st = _tokens(op, "query", query, cu_q)
+        q_shape = query.shape
+        if q_shape[:-2] != shape[:-2] or q_shape[-1] != D or query.dtype is not dtype:
+            raise RuntimeError(f"{op}: query {tuple(q_shape)} {query.dtype} does not match key {tuple(shape)} {dtype}")
         if query_out is None:
-            query_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-        elif query_out.shape != query.shape or query_out.dtype != query.dtype:
+            query_out = torch.empty_like(query)
+        elif query_out.shape != q_shape or query_out.dtype is not dtype:
             raise RuntimeError(f"{op}: query_out must match query in shape and dtype")
-        _, _, _, o_st = _tokens("query_out", query_out, cu_q)
-        Hq = query.shape[-2]
+        o_st = _tokens(op, "query_out", query_out, cu_q)
+        Hq, q_ptr, o_ptr = q_shape[-2], query.data_ptr(), query_out.data_ptr()
     elif query_out is not None:
         raise RuntimeError(f"{op}: query_out without a query")
-    if rope_theta is not None and not rope_theta > 0:
-        raise RuntimeError(f"{op}: rope_theta must be > 0 (got {rope_theta})")
-    strides = _lib.int64_array([*q_st, *k_st, *v_st, *o_st, *k_pages.stride()[:3], *v_pages.stride()[:3],
-                                block_table.stride(0)])
-    _lib.call("dgg_paged_append", _lib.ptr(query), _lib.ptr(key), _lib.ptr(value), _lib.ptr(query_out),
-              _lib.ptr(k_pages), _lib.ptr(v_pages), _lib.ptr(block_table), _lib.ptr(kv_lens), _lib.ptr(cu_q), B, T, Sq,
-              Hq, Hkv, D, n_pages, page, block_table.shape[1], strides, float(rope_theta or 0.0),
-              _lib.dtype_code(key.dtype), _lib.stream_handle(dev))
+    strides = _STRIDES_19.pack(*q_st, *k_st, *v_st, *o_st, *pool_st, block_table.stride(0))
+    _lib.call("dgg_paged_append", q_ptr, key.data_ptr(), value.data_ptr(), o_ptr, k_pages.data_ptr(),
+              v_pages.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), _lib.ptr(cu_q), B, T, Sq, Hq, Hkv, D,
+              n_pages, page, width, strides, rope_theta or 0.0, _lib.dtype_code(dtype), _lib.stream_handle(dev))
     return query_out
 
 
 def _attend(op: str, q, k_pages, v_pages, block_table, kv_lens, prefix_len, cu_q, causal, softcap, window, scale,
             return_lse, out):
-    dev = _lib.require_gpu(q, k_pages, v_pages, block_table, kv_lens, cu_q, out)
-    _check_cu(op, cu_q)
-    B, T, Sq, q_st = _tokens("q", q, cu_q)
-    _cache(op, k_pages, v_pages, block_table, kv_lens, cu_q, B)
-    n_pages, page, Hkv, D = k_pages.shape
-    Hq = q.shape[-2]
-    if q.shape[-1] != D or q.dtype != k_pages.dtype:
-        raise RuntimeError(f"{op}: q {tuple(q.shape)} {q.dtype} does not match pages {tuple(k_pages.shape)} "
-                           f"{k_pages.dtype}")
+    dev = _device(q, k_pages, v_pages, block_table, kv_lens, cu_q, out)
+    q_st = _tokens(op, "q", q, cu_q)
+    B, T, Sq = _batch(op, q, cu_q)
+    (n_pages, page, Hkv, D), width, pool_st = _cache(op, k_pages, v_pages, block_table, kv_lens, cu_q, B)
+    shape, dtype = q.shape, q.dtype
+    Hq = shape[-2]
+    if shape[-1] != D or dtype is not k_pages.dtype:
+        raise RuntimeError(f"{op}: q {tuple(shape)} {dtype} does not match pages {tuple(k_pages.shape)} {k_pages.dtype}")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype:
+        out = torch.empty_like(q)
+    elif out.shape != shape or out.dtype is not dtype:
         raise RuntimeError(f"{op}: out must match q in shape and dtype")
-    _, _, _, o_st = _tokens("out", out, cu_q)
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    need = _lib.load().dgg_attn_paged_workspace_bytes(B, T, Sq, Hq, Hkv, D, int(prefix_len))
-    if need < 0:
-        raise RuntimeError(f"{op}: {_lib.load().dgg_last_error().decode(errors='replace')}")
-    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+    o_st = _tokens(op, "out", out, cu_q)
+    ws_bytes = _workspace_bytes(op, B, T, Sq, Hq, Hkv, D, prefix_len)
+    ws = q.new_empty(ws_bytes // 2 + 8)  # (of 16-bit elements; another type is refused below)
     lse = torch.empty(T, Hq, dtype=torch.float32, device=q.device) if return_lse else None
-    strides = _lib.int64_array([*q_st, *k_pages.stride()[:3], *v_pages.stride()[:3], *o_st, block_table.stride(0)])
-    _lib.call("dgg_attn_paged", _lib.ptr(q), _lib.ptr(k_pages), _lib.ptr(v_pages), _lib.ptr(out), _lib.ptr(lse),
-              _lib.ptr(block_table), _lib.ptr(kv_lens), _lib.ptr(cu_q), _lib.ptr(ws), ws.numel(), B, T, Sq, Hq, Hkv, D,
-              n_pages, page, block_table.shape[1], int(prefix_len), strides, scale, float(softcap or 0.0),
-              int(window or 0), _lib.ATTN_CAUSAL if causal else 0, _lib.dtype_code(q.dtype), _lib.stream_handle(dev))
+    strides = _STRIDES_13.pack(*q_st, *pool_st, *o_st, block_table.stride(0))
+    _lib.call("dgg_attn_paged", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), _lib.ptr(lse),
+              block_table.data_ptr(), kv_lens.data_ptr(), _lib.ptr(cu_q), ws.data_ptr(), ws_bytes, B, T, Sq, Hq, Hkv, D,
+              n_pages, page, width, prefix_len, strides, 1.0 / math.sqrt(D) if scale is None else scale, softcap or 0.0,
+              window or 0, _lib.ATTN_CAUSAL if causal else 0, _lib.dtype_code(dtype), _lib.stream_handle(dev))
     if not return_lse:
         return out
     return out, lse if cu_q is not None else lse.view(B, Sq, Hq).transpose(1, 2)
@@ -167,9 +187,5 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     of block_table are not looked at there), the rest of each sequence from its own pages, and the two are joined
     by their log-sum-exp. prefix_len is a number of whole pages; kv_lens and positions count the prefix. Results and other
     arguments as paged_attention(), which computes the same from tables that repeat the prefix's pages."""
-    prefix_len, page = int(prefix_len), k_pages.shape[1] if k_pages.dim() == 4 else 1
-    if prefix_len < 0 or prefix_len % max(page, 1) or prefix_len > block_table.shape[-1] * page:
-        raise RuntimeError(f"shared_prefix_attention: prefix_len {prefix_len} must be whole pages of {page} keys that the "
-                           "block table names")
-    return _attend("shared_prefix_attention", q, k_pages, v_pages, block_table, kv_lens, prefix_len, cu_q, causal,
+    return _attend("shared_prefix_attention", q, k_pages, v_pages, block_table, kv_lens, int(prefix_len), cu_q, causal,
                    softcap, window, scale, return_lse, out)
