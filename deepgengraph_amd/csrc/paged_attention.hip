@@ -265,16 +265,18 @@ struct State {
 
 constexpr int kOQ = 64 * 16 + 16;  // a quad of O registers of a wave in the LDS, and padding
 
-// Leaves a wave's state in its slot: D / 8 quads of O, and (maximum in the exp2 domain, sum) of each row.
+// Leaves a wave's state in its slot: D / 8 quads of O, and (maximum in the exp2 domain, sum) of each row. ok: the lane has
+// a row (lanes without one would take their turns at the LDS, too).
 template <int D>
-__device__ __forceinline__ void put_state(const State<D>& st, char* slot, f32x2* ml, float c, int lane) {
+__device__ __forceinline__ void put_state(const State<D>& st, char* slot, f32x2* ml, float c, int lane, bool ok) {
+  const float l = half_swap_sum(st.l[0] + st.l[1]);
+  if (!ok) return;
 #pragma unroll
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
     for (int jj = 0; jj < 4; ++jj)
       *reinterpret_cast<f32x4*>(slot + (db * 4 + jj) * kOQ + lane * 16) =
           f32x4{st.o[db][4 * jj], st.o[db][4 * jj + 1], st.o[db][4 * jj + 2], st.o[db][4 * jj + 3]};
-  const float l = half_swap_sum(st.l[0] + st.l[1]);
   if (lane < 32) ml[lane] = f32x2{st.m == -INFINITY ? -INFINITY : st.m * c, l};
 }
 
@@ -394,8 +396,6 @@ __device__ __forceinline__ void narrow_unit(const Unit& u, char* smem, int hk, i
   GranuleCopy<D, true> kc, vc;
   kc.init(lane, k_ss_b);
   vc.init(lane, v_ss_b);
-  Fragments<D> fr;
-  fr.init(lane, wave_at, wave_at + TILE_B);
   const char* kp = static_cast<const char*>(p.k) + 2 * hk * p.k_sh;
   const char* vp = static_cast<const char*>(p.v) + 2 * hk * p.v_sh;
 
@@ -417,10 +417,6 @@ __device__ __forceinline__ void narrow_unit(const Unit& u, char* smem, int hk, i
   };
   auto holes_of = [&](int s) { return ~(unsigned)(gr.live >> (2 * (s & 31))) & 3u; };
 
-  const Seen see = seen_by_wave(p, u, x, u.row0);
-  State<D> st;
-  st.init();
-  const float c = score_coeff<SOFTCAP, 0>(p.s);
   unsigned holes = 0;
   if (n_own > 0) {
     gr.take(p, u, mine.granule(0), mine.granule(32));
@@ -429,6 +425,13 @@ __device__ __forceinline__ void narrow_unit(const Unit& u, char* smem, int hk, i
     holes = holes_of(0);
   }
   ahead();
+  // (what the first tile needs besides, while it is on its way)
+  Fragments<D> fr;
+  fr.init(lane, wave_at, wave_at + TILE_B);
+  const Seen see = seen_by_wave(p, u, x, u.row0);
+  State<D> st;
+  st.init();
+  const float c = score_coeff<SOFTCAP, 0>(p.s);
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk) {
     asm volatile("" : "+v"(qf[kk]));
@@ -494,7 +497,7 @@ __device__ __forceinline__ void narrow_unit(const Unit& u, char* smem, int hk, i
   char* slots = smem;
   f32x2* ml = reinterpret_cast<f32x2*>(smem + NW * WAVE_B);
   wait_vmem<0>();
-  put_state(st, slots + w * WAVE_B, ml + 32 * w, c, lane);
+  put_state(st, slots + w * WAVE_B, ml + 32 * w, c, lane, x.ok);
   __syncthreads();
   const PagedParams& pe = fresh_params();
   const int items = min(32, u.rows - u.row0) * (D / 8);
@@ -637,8 +640,6 @@ __device__ __forceinline__ void wide_unit(const Unit& u, char* smem, int hk) {
   GranuleCopy<D, false> kc, vc;
   kc.init(lane, k_ss_b);
   vc.init(lane, v_ss_b);
-  Fragments<D> fr;
-  fr.init(lane, smem_at + (koff / L::GR) * L::GROUP_B, smem_at + TILE_B + (koff / L::GR) * L::GROUP_B);
   const char* kp = static_cast<const char*>(p.k) + 2 * hk * p.k_sh;
   const char* vp = static_cast<const char*>(p.v) + 2 * hk * p.v_sh;
 
@@ -676,15 +677,18 @@ __device__ __forceinline__ void wide_unit(const Unit& u, char* smem, int hk) {
     }
   };
 
-  const Seen see = seen_by_wave(p, u, x, u.row0 + 32 * wr);
-  State<D> st;
-  st.init();
-  const float c = score_coeff<SOFTCAP, 0>(p.s);
   if (t_first < t_end) {
     gr.take(p, u, gran_of(t_first), gran_of(t_first + WINDOW));
     aim(t_first);
     issue(t_first);
   }
+  // (what the first tile needs besides, while it is on its way)
+  Fragments<D> fr;
+  fr.init(lane, smem_at + (koff / L::GR) * L::GROUP_B, smem_at + TILE_B + (koff / L::GR) * L::GROUP_B);
+  const Seen see = seen_by_wave(p, u, x, u.row0 + 32 * wr);
+  State<D> st;
+  st.init();
+  const float c = score_coeff<SOFTCAP, 0>(p.s);
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk) {
     if (!x.ok) qf[kk] = V8{};
@@ -812,7 +816,7 @@ __device__ __forceinline__ void wide_unit(const Unit& u, char* smem, int hk) {
   // States go through the LDS, so that the stores cover whole rows; KG states of a row are joined.
   f32x2* ml = reinterpret_cast<f32x2*>(smem + NW * SLOT_B);
   __syncthreads();  // every wave is done with the tiles
-  put_state(st, smem + w * SLOT_B, ml + 32 * w, c, lane);
+  put_state(st, smem + w * SLOT_B, ml + 32 * w, c, lane, x.ok);
   __syncthreads();
   const PagedParams& pe = fresh_params();
   // Each wave writes a KG-th of the rows that it holds.
