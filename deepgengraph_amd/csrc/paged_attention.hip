@@ -862,20 +862,23 @@ paged_mixed_kernel(PagedParams p) {
 }
 
 // Joins the partials of rows: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, lse = (M + log2 L) ln 2, with those of the
-// prefix first and then the sequence's own. A workgroup takes rows_per_merge rows of the batch (token-major, as the prefix
-// numbers them) of a KV head. Its groups of D / 4 threads (four head-dim elements each) take rows, or, where a row has many
-// partials, share one.
-constexpr int kMergeThreads = 256;
-template <typename T, int D, bool WIDE>
-__global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(PagedParams p) {
+// prefix first and then the sequence's own. A wave takes rows_per_merge rows of the batch (token-major, as the prefix numbers
+// them) of a KV head, by itself: its time is the chain lengths -> partials -> output, once for each sequence that its rows
+// touch. Its groups of D / 4 lanes (four head-dim elements each) take rows in turn, or share one of many partials. TEAM: the
+// four waves of a workgroup share one row, where there are few.
+constexpr int kMergeWaves = 4;
+template <typename T, int D, bool WIDE, bool TEAM>
+__global__ void __launch_bounds__(64 * kMergeWaves) paged_merge_kernel(PagedParams p) {
   typedef typename T::scalar S;
   typedef typename T::vec4 V4;
-  constexpr int COLS = D / 4, NG = kMergeThreads / COLS;
-  __shared__ f32x4 part[NG][COLS];
-  __shared__ f32x2 part_ml[NG];
-  const int tid = threadIdx.x, lane = tid & 63, col = tid % COLS, grp = tid / COLS;
-  const int hk = blockIdx.x % p.Hkv;
-  const int from = blockIdx.x / p.Hkv * p.rows_per_merge, to = min(p.T * p.G, from + p.rows_per_merge);
+  constexpr int COLS = D / 4, NG = 64 / COLS;
+  const int lane = threadIdx.x & 63, col = lane % COLS, grp = lane / COLS;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = TEAM ? blockIdx.x : blockIdx.x * kMergeWaves + w;
+  __shared__ f32x4 team_o[TEAM ? kMergeWaves : 1][COLS];
+  __shared__ f32x2 team_ml[TEAM ? kMergeWaves : 1];
+  const int hk = wave % p.Hkv;
+  const int from = wave / p.Hkv * p.rows_per_merge, to = min(p.T * p.G, from + p.rows_per_merge);
   const Division d = divide<WIDE>(p, lane);
   for (int f = from; f < to;) {
     const Place pl = find_place<WIDE, kToken>(p, d, f / p.G, lane);
@@ -900,14 +903,11 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(PagedParams 
     if (p.P == 0 && n_own == 1) continue;  // written by its unit
     const int last_slot = own0 + (wide ? (row_groups(p, pl.s.n * p.G) - 1) * n_own : 0) + n_own - 1;
     if (last_slot >= (wide ? p.wide_slots : p.narrow_slots)) return;  // (only where cu_q descends)
-    int shared = 0;  // log2 of the groups that share a row
-    while ((1 << shared) < NG && (n_all >> shared) > 4 && (NG >> shared) > 1 &&
-           ((NG >> shared) > r_to - r_from || (n_all >> shared) > 8))
-      ++shared;
-    const int sub = grp & ((1 << shared) - 1), step = 1 << shared, rows_at_once = NG >> shared;
-    for (int r0 = r_from; r0 < r_to; r0 += rows_at_once) {
-      const int row = r0 + (grp >> shared);
-      const bool ok = row < r_to;
+    const bool share = NG > 1 && (TEAM || n_all > 8 || r_to - r_from < NG);  // all groups on one row
+    const int sub = (share ? grp : 0) + (TEAM ? w * NG : 0), step = (share ? NG : 1) * (TEAM ? kMergeWaves : 1);
+    const int at_once = share ? 1 : NG;
+    for (int r0 = r_from; r0 < r_to; r0 += at_once) {
+      const int row = r0 + (share ? 0 : grp);
       const int rc = min(row, r_to - 1);
       const int qi = rc / p.G, qg = rc - qi * p.G, tok = pl.s.t0 + qi, h = hk * p.G + qg;
       const int prow = tok * p.G + qg;
@@ -921,59 +921,76 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(PagedParams 
         pm = (w ? p.wide_ml : p.narrow_ml) + at * 2;
       };
       const int rg = rc >> p.log2_r, prg = prow >> p.log2_r, rmask = (1 << p.log2_r) - 1;
-      locate(wide, own0 + (wide ? rg * n_own : 0), wide ? rc & rmask : rc, own_o, own_ml, own_step);
       const bool pw = WIDE && p.prefix_wide;
+      locate(wide, own0 + (wide ? rg * n_own : 0), wide ? rc & rmask : rc, own_o, own_ml, own_step);
       locate(pw, pw ? prg * d.p_ns : 0, pw ? prow & rmask : prow, pre_o, pre_ml, pre_step);
       float M = -INFINITY, Ls = 0.f;
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-      constexpr int U = 4;  // partials in flight
-      for (int i0 = sub; i0 < n_all; i0 += step * U) {
-        f32x4 o[U];
-        f32x2 x[U];
+      auto sweep = [&](auto in_flight) __attribute__((always_inline)) {
+        constexpr int U = decltype(in_flight)::value;
+        for (int i0 = sub; i0 < n_all; i0 += step * U) {
+          f32x4 o[U];
+          f32x2 x[U];
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-          const int i = min(i0 + step * k, n_all - 1);
-          const bool pre = i < n_pre;
-          const int64_t at = pre ? i * pre_step : (i - n_pre) * own_step;
-          x[k] = *reinterpret_cast<const f32x2*>((pre ? pre_ml : own_ml) + 2 * at);
-          o[k] = *reinterpret_cast<const f32x4*>((pre ? pre_o : own_o) + at * D);
-        }
-        float m = M;
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-          if (i0 + step * k >= n_all) x[k] = f32x2{-INFINITY, 0.f};
-          m = fmaxf(m, x[k][0]);
-        }
-        const float mu = m == -INFINITY ? 0.f : m, a = fast_exp2(M - mu);
-        acc *= a;
-        Ls *= a;
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-          const float wgt = fast_exp2(x[k][0] - mu);
-          acc += wgt * o[k];
-          Ls = fmaf(wgt, x[k][1], Ls);
-        }
-        M = m;
-      }
-      if (shared > 0) {
-        part[grp][col] = acc;
-        if (col == 0) part_ml[grp] = f32x2{M, Ls};
-        __syncthreads();
-        if (sub == 0) {
-          M = -INFINITY;
-          for (int i = 0; i < step; ++i) M = fmaxf(M, part_ml[grp + i][0]);
-          const float mu = M == -INFINITY ? 0.f : M;
-          Ls = 0.f;
-          acc = f32x4{0.f, 0.f, 0.f, 0.f};
-          for (int i = 0; i < step; ++i) {
-            const float wgt = fast_exp2(part_ml[grp + i][0] - mu);
-            Ls = fmaf(wgt, part_ml[grp + i][1], Ls);
-            acc += wgt * part[grp + i][col];
+          for (int k = 0; k < U; ++k) {
+            const int i = min(i0 + step * k, n_all - 1);
+            const bool pre = i < n_pre;
+            const int64_t at = pre ? i * pre_step : (i - n_pre) * own_step;
+            x[k] = *reinterpret_cast<const f32x2*>((pre ? pre_ml : own_ml) + 2 * at);
+            o[k] = *reinterpret_cast<const f32x4*>((pre ? pre_o : own_o) + at * D);
           }
+          float m = M;
+#pragma unroll
+          for (int k = 0; k < U; ++k) {
+            if (i0 + step * k >= n_all) x[k] = f32x2{-INFINITY, 0.f};
+            m = fmaxf(m, x[k][0]);
+          }
+          const float mu = m == -INFINITY ? 0.f : m, a = fast_exp2(M - mu);
+          acc *= a;
+          Ls *= a;
+#pragma unroll
+          for (int k = 0; k < U; ++k) {
+            const float wgt = fast_exp2(x[k][0] - mu);
+            acc += wgt * o[k];
+            Ls = fmaf(wgt, x[k][1], Ls);
+          }
+          M = m;
         }
-        __syncthreads();
+      };
+      if (n_all > 4 * step) sweep(std::integral_constant<int, 16>{});
+      else sweep(std::integral_constant<int, 4>{});
+      if (share) {  // (the groups' states, exchanged among lanes of the same elements)
+#pragma unroll
+        for (int off = COLS; off < 64; off <<= 1) {
+          const float m2 = __shfl_xor(M, off, 64), l2 = __shfl_xor(Ls, off, 64);
+          f32x4 o2;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o2[e] = __shfl_xor(acc[e], off, 64);
+          const float m = fmaxf(M, m2), mu = m == -INFINITY ? 0.f : m;
+          const float wa = fast_exp2(M - mu), wb = fast_exp2(m2 - mu);
+          acc = acc * wa + o2 * wb;
+          Ls = Ls * wa + l2 * wb;
+          M = m;
+        }
       }
-      if (!ok || sub != 0) continue;
+      if constexpr (TEAM) {  // (rows_per_merge is 1: once)
+        if (grp == 0) team_o[w][col] = acc;
+        if (lane == 0) team_ml[w] = f32x2{M, Ls};
+        __syncthreads();
+        M = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kMergeWaves; ++i) M = fmaxf(M, team_ml[i][0]);
+        const float mu = M == -INFINITY ? 0.f : M;
+        acc = f32x4{0.f, 0.f, 0.f, 0.f};
+        Ls = 0.f;
+#pragma unroll
+        for (int i = 0; i < kMergeWaves; ++i) {
+          const float wgt = fast_exp2(team_ml[i][0] - mu);
+          acc += wgt * team_o[i][col];
+          Ls = fmaf(wgt, team_ml[i][1], Ls);
+        }
+      }
+      if (row >= r_to || sub != 0) continue;
       const float inv = Ls == 0.f ? 0.f : 1.0f / Ls;
       S* op = static_cast<S*>(p.o) + (p.cu_q != nullptr ? tok * p.o_ss : pl.b * p.o_sb + qi * p.o_ss) + h * p.o_sh;
       V4 ov;
@@ -1057,11 +1074,18 @@ void launch(const PagedParams& p, hipStream_t st) {
   if (p.s.softcap > 0.f) launch_cap<T, D, true>(p, st);
   else launch_cap<T, D, false>(p, st);
   const int64_t rows = (int64_t)p.T * p.G;
-  const int64_t wgs = (rows + p.rows_per_merge - 1) / p.rows_per_merge * p.Hkv;
-  if (p.wide_units > 0)
-    hipLaunchKernelGGL((paged_merge_kernel<T, D, true>), dim3((unsigned)wgs), dim3(kMergeThreads), 0, st, p);
-  else
-    hipLaunchKernelGGL((paged_merge_kernel<T, D, false>), dim3((unsigned)wgs), dim3(kMergeThreads), 0, st, p);
+  const int64_t waves = (rows + p.rows_per_merge - 1) / p.rows_per_merge * p.Hkv;
+  // A workgroup per row up to 512 rows: two per CU (8 sequences of one token behind a prefix of 8,192, 256 rows of up to 66
+  // partials: 22.5 us against 25.4 with a wave for each; 64 sequences, 2,048 rows: 297 against 293).
+  const bool team = rows * p.Hkv <= 512;
+  const dim3 grid((unsigned)(team ? waves : (waves + kMergeWaves - 1) / kMergeWaves)), block(64 * kMergeWaves);
+  if (p.wide_units > 0) {
+    if (team) hipLaunchKernelGGL((paged_merge_kernel<T, D, true, true>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((paged_merge_kernel<T, D, true, false>), grid, block, 0, st, p);
+  } else {
+    if (team) hipLaunchKernelGGL((paged_merge_kernel<T, D, false, true>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((paged_merge_kernel<T, D, false, false>), grid, block, 0, st, p);
+  }
 }
 
 int check_sizes(const char* op, int64_t B, int64_t T, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix) {
@@ -1187,7 +1211,7 @@ extern "C" int dgg_attn_paged(const void* q, const void* k_pages, const void* v_
   p.narrow_slots = h.narrow_slots;
   p.narrow_rows = h.narrow_rows;
   p.per_wide = h.wide_target > 0 ? (float)((1.0 + 1.0 / 2048) / h.wide_target) : 0.f;
-  p.rows_per_merge = (int)std::max<int64_t>(1, T * p.G * Hkv / 2048);
+  p.rows_per_merge = (int)std::max<int64_t>(1, T * p.G * Hkv / 4096);
   hipStream_t st = dgg::as_stream(stream);
   if (dtype == DGG_BF16) {
     if (D == 64) launch<BF16, 64>(p, st);
