@@ -44,8 +44,7 @@ EXTRA_FLAGS = {
     for name in ("attention.hip", "attention_fwd_f16.hip", "attention_fwd_bf16.hip", "attention_d256.hip")
 }
 
-# (and of these the wide units 1 to 2%; both options together do not compile there)
-EXTRA_FLAGS["paged_attention.hip"] = ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"]
+EXTRA_FLAGS.update({f"paged_attention_d{d}.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"] for d in (64, 128, 256)})
 
 
 def _hipcc() -> str:

@@ -60,6 +60,11 @@ struct PagedParams {
   dgg_attn::AttnParams s;   // scale and soft-cap constants (score_value)
 };
 
+// Launch the kernels for p (paged_attention_d*.hip).
+void launch_d64(const PagedParams& p, bool bf16, hipStream_t st);
+void launch_d128(const PagedParams& p, bool bf16, hipStream_t st);
+void launch_d256(const PagedParams& p, bool bf16, hipStream_t st);
+
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
