@@ -6,7 +6,8 @@ attention -> output projection. The projections are plain library GEMMs (torch.m
 else runs in libdgg_hip.so. Unlike the reference, q/k/v are not copied out of the QKV result with
 .contiguous() (models/attn.py:36-39): the rotary and attention kernels take the strided views directly. With
 fuse_rope (head_dim 128) the query's rotation runs inside the attention kernel from a per-position (cos, sin)
-table, and the rotary kernel rotates k only: the query never makes the extra round trip through HBM.
+table, and the rotary kernel rotates k only: the query never makes the extra round trip through HBM. paged_step is
+the block over a paged key/value cache, for prompt chunks and decode steps of a ragged batch.
 """
 from __future__ import annotations
 
@@ -14,6 +15,7 @@ import torch
 
 from . import attention as _attn
 from . import ops
+from . import paged as _paged
 
 
 class LlamaAttentionBlock:
@@ -60,6 +62,24 @@ class LlamaAttentionBlock:
             ops.rotary_embedding_online(pos, q, k, D, self.theta)     # models/attn.py:41
             o = _attn.attention(q.view(B, S, H, D), k.view(B, S, Hk, D), v.view(B, S, Hk, D), causal=True)
         return torch.matmul(o.view(B, S, H * D), self.w_o.t())         # models/attn.py:52
+
+    def paged_step(self, x: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                   kv_lens: torch.Tensor, *, cu_q: torch.Tensor | None = None, prefix_len: int = 0) -> torch.Tensor:
+        """The block as a server runs it: the step's tokens x [B, Sq, hidden] (or [T, hidden] with cu_q) against the
+        sequences' paged cache (deepgengraph_amd.paged), into which their keys and values go. kv_lens count this
+        step's tokens; prefix_len: keys that all sequences share, in whole pages (the step's own lie behind them).
+        Prompt chunks and decode steps alike; the serving counterpart of __call__, which keeps no cache."""
+        D, H, Hk = self.head_dim, self.heads, self.kv_heads
+        h = torch.empty_like(x)
+        ops.rms_norm(h, x, self.w_norm, self.eps)
+        q, k, v = (t.unflatten(-1, (-1, D)) for t in
+                   torch.matmul(h, self.w_qkv.t()).split([H * D, Hk * D, Hk * D], dim=-1))
+        q = _paged.paged_append(k, v, k_pages, v_pages, block_table, kv_lens, query=q, cu_q=cu_q, rope_theta=self.theta)
+        if prefix_len:
+            o = _paged.shared_prefix_attention(q, k_pages, v_pages, block_table, kv_lens, prefix_len, cu_q=cu_q)
+        else:
+            o = _paged.paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q=cu_q)
+        return torch.matmul(o.flatten(-2), self.w_o.t())
 
 
 def decode_prestep(x: torch.Tensor, w_norm: torch.Tensor, gate_up: torch.Tensor, eps: float = 1e-6):

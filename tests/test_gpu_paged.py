@@ -171,6 +171,35 @@ def test_prefix_that_covers_everything(gpu):
     _run(gpu, [600, 540], [30, 2], prefix=512, causal=False)
 
 
+@pytest.mark.parametrize("heads", [(256, 256), (256, 128)])
+def test_large_row_groups(gpu, heads):
+    # chunks that fill the chip run in row groups of 256
+    q = 256 * 256 // heads[1] * heads[1] // heads[0]
+    _run(gpu, [q + 137], [q], Hq=heads[0], Hkv=heads[1], seed=heads[1])
+    _run(gpu, [300, 129], [128, 128], Hq=heads[0], Hkv=heads[1], dtype=torch.float16, window=90)
+
+
+def test_row_groups_cut_and_uncut(gpu):
+    # uneven chunks whose row groups nearly fill the chip, so that only the longest are cut; and long ones among short
+    _run(gpu, [130 * (b % 3 + 1) for b in range(24)], [100] * 24, Hq=8, Hkv=8, D=64)
+    _run(gpu, [2000, 70, 65, 900], [65, 70, 65, 33], Hq=4, Hkv=1, D=256, dtype=torch.float16)
+    _run(gpu, [40, 2100], [33, 34], Hq=2, Hkv=1)
+
+
+def test_most_sequences(gpu):
+    # the most that a call takes: each lane looks at 64 of them
+    kv = [(b * 7) % 33 for b in range(4096)]
+    _run(gpu, kv, [1] * 4096, Hq=1, Hkv=1, D=64)
+    n = [0 if b % 5 == 1 else 1 + (b % 7 == 3) * 2 for b in range(1000)]
+    n[500] = 60
+    _run(gpu, [max(k, m) for k, m in zip(kv, n)], n, Hq=2, Hkv=1, D=64, ragged=True, tail=3)
+
+
+def test_prefix_with_many_sequences(gpu):
+    _run(gpu, [96 + b % 40 for b in range(130)], [1] * 130, prefix=96, Hq=2, Hkv=1, D=64)
+    _run(gpu, [96 + b % 40 for b in range(130)], [b % 3 for b in range(130)], prefix=96, Hq=2, Hkv=2, D=64)
+
+
 def test_prefix_is_the_first_sequences(gpu):
     # the other rows of the table are not looked at inside the prefix
     g = _gen(5)
@@ -380,6 +409,70 @@ def test_refusals(gpu):
     assert at(q[:, :0], kd, vd, td, ld).shape == (2, 0, 4, 64)
     # without pages nobody has a key
     assert (at(q, kd[:0], vd[:0], td, ld) == 0).all()
+
+
+def test_two_streams(gpu):
+    """Calls on two streams at once, each with a workspace of its own, give what they give one after the other."""
+    g = _gen(31)
+    kv = [700, 90, 1500, 33]
+    kp, vp, table = _cache(g, kv, 16, 2, 128, torch.bfloat16)
+    args = _to(gpu, kp, vp, table, kv)
+    qs = [torch.randn(4, n, 8, 128, generator=g).bfloat16().to(gpu) for n in (1, 24)]
+    want = [paged.paged_attention(q, *args) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(paged.paged_attention(qs[i], *args))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in got[i])
+
+
+@pytest.mark.parametrize("prefix", [0, 32])
+def test_llama_block_over_a_paged_cache(gpu, prefix):
+    """A prompt in uneven chunks, then decode steps, through the attention block: with the identity as its output
+    projection the block returns the attention of the projected rows, which the 64-bit oracle computes from the same
+    projections (the norm and the projection are the block's own, tested elsewhere)."""
+    from deepgengraph_amd import llama, ops
+
+    g = _gen(17)
+    B, H, Hk, D, page, width = 3, 4, 2, 128, 16, 8
+    hidden = H * D
+    w_norm = (1 + 0.02 * torch.randn(hidden, generator=g)).bfloat16().to(gpu)
+    w_qkv = (0.05 * torch.randn(hidden + 2 * Hk * D, hidden, generator=g)).bfloat16().to(gpu)
+    block = llama.LlamaAttentionBlock(w_norm, w_qkv, torch.eye(hidden).bfloat16().to(gpu), heads=H, kv_heads=Hk)
+    table = torch.randperm(B * width, generator=g).view(B, width).to(torch.int32)
+    if prefix:
+        table[1:, : prefix // page] = table[0, : prefix // page]
+    kp = torch.randn(B * width, page, Hk, D, generator=g).bfloat16()
+    vp = torch.randn(B * width, page, Hk, D, generator=g).bfloat16()
+    kd, vd, td = kp.to(gpu), vp.to(gpu), table.to(gpu)
+    lens = [prefix] * B
+    for n in ([20, 1, 33], [1, 30, 2], [1, 1, 1], [1, 1, 1]):
+        lens = [a + b for a, b in zip(lens, n)]
+        ld = torch.tensor(lens, dtype=torch.int32, device=gpu)
+        same = len(set(n)) == 1
+        cu = None if same else torch.tensor([0, n[0], n[0] + n[1], sum(n)], dtype=torch.int32)
+        x = torch.randn(*((B, n[0]) if same else (sum(n),)), hidden, generator=g).bfloat16().to(gpu)
+        y = block.paged_step(x, kd, vd, td, ld, cu_q=None if cu is None else cu.to(gpu), prefix_len=prefix)
+        h = torch.empty_like(x)
+        ops.rms_norm(h, x, w_norm, block.eps)
+        q, k, v = (t.unflatten(-1, (-1, D)) for t in
+                   torch.matmul(h, w_qkv.t()).cpu().split([hidden, Hk * D, Hk * D], dim=-1))
+        rk, rv, rq = op.append(k, v, kp, vp, table, lens, query=q, cu_q=cu, rope_theta=1e4)
+        _same_pool(kd, rk, 2 ** -8, f"keys {n}")
+        _same_pool(vd, rv, 0, f"values {n}")
+        kp, vp = kd.cpu(), vd.cpu()
+        # the query that the attention saw (the same rows are stored once more)
+        qd, kd2, vd2 = (t.to(gpu) for t in (q, k, v))
+        seen = paged.paged_append(kd2, vd2, kd, vd, td, ld, query=qd, cu_q=None if cu is None else cu.to(gpu),
+                                  rope_theta=1e4).cpu()
+        _same_pool(seen, rq, 2 ** -8, f"queries {n}")
+        ref = op.attention(seen, kp, vp, table, lens, cu_q=cu, prefix_len=prefix)
+        _check(y.unflatten(-1, (H, D)), None, ref, f"step {n}")
 
 
 def test_step_together_captured(gpu):
