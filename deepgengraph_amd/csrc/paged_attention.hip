@@ -25,8 +25,9 @@ struct HostPlan {
 // step at 256, 384, 448, 512 units 138, 136, 135, 131; 8 chunks of up to 1,024 tokens 148, 147, 147, 158; the prefix of
 // 16,384 133, 106, 101, 100).
 // Narrow stretches: one for each resident workgroup, of at most two per CU (32 x 16 heads of 64, up to 4,000 keys: 512
-// stretches 53, 768 56); beside wide units three quarters of them, so that both begin at once
-// (the step at 256, 384, 512 stretches 138, 137, 157).
+// stretches 53, 768 56). Beside wide units one per CU: that many saturate the memory, and more only lengthen the latency
+// that the wide units see (the step of 28 decode rows and 4 chunks at 128, 256, 384 stretches 129, 127, 132, 64 decode rows
+// behind a prefix of 8,192 77, 55, 55).
 HostPlan host_plan(int64_t B, int64_t T, bool ragged, int64_t Hq, int64_t Hkv, int64_t D, int64_t P) {
   HostPlan h{};
   const int64_t G = Hq / Hkv, Sq = T / B, CUs = 256;
@@ -50,7 +51,7 @@ HostPlan host_plan(int64_t B, int64_t T, bool ragged, int64_t Hq, int64_t Hkv, i
     h.wide_rows = (int)std::min<int64_t>(R, h.prefix_wide ? T * G : most);
   }
   if (narrow) {
-    h.narrow_wgs = (int)std::max<int64_t>(1, (wide ? CUs * per_cu * 3 / 4 : CUs * std::min<int64_t>(per_cu, 2)) / Hkv);
+    h.narrow_wgs = (int)std::max<int64_t>(1, (wide ? std::min(CUs, CUs * per_cu * 3 / 4) : CUs * std::min<int64_t>(per_cu, 2)) / Hkv);
     h.narrow_slots = (int)(h.narrow_wgs + B + 1);
     h.narrow_rows = (int)std::min<int64_t>(dgg_paged::kNarrowRows, P > 0 && !h.prefix_wide ? T * G : most);
   }
