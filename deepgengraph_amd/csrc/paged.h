@@ -141,6 +141,7 @@ struct Division {
   int p_tiles;       // narrow prefix: tiles
   int stretch;       // tiles of a narrow workgroup
   int tiles;         // all narrow tiles
+  bool invalid;      // the lengths make no sense
   // per lane: the last of its sequences, and its own and the running number of narrow tiles, wide units, partial slots
   Seq s;
   int my_tiles, my_units, my_slots, run_tiles, run_units, run_slots;
@@ -169,6 +170,7 @@ template <bool WIDE>
 __device__ __forceinline__ Division divide(const PagedParams& p, int lane) {
   const int c = (p.B + 63) >> 6;
   float work = 0.f, groups = 0.f;  // (32 bits do: the quotient is rounded up, and every wave adds in the same order)
+  float tokens = 0.f;              // (fewer than 2^24: exact)
   int lo = p.P;
   Division d{};
   for (int j = 0; j < c; ++j) {
@@ -176,6 +178,7 @@ __device__ __forceinline__ Division divide(const PagedParams& p, int lane) {
     if (b >= p.B) break;
     d.s = load_seq(p, b);
     if (d.s.n == 0) continue;
+    tokens += (float)d.s.n;
     if (!is_wide(p, d.s)) d.my_tiles += seq_tiles(p, d.s);
     else if (WIDE) {
       const float nrg = (float)row_groups(p, d.s.n * p.G);
@@ -183,6 +186,13 @@ __device__ __forceinline__ Division divide(const PagedParams& p, int lane) {
       work += nrg * (float)seq_tiles(p, d.s);
     }
     lo = min(lo, p.window > 0 ? max(0, d.s.kv - d.s.n - p.window + 1) : 0);
+  }
+  // A cu_q that descends can name a token more than once, and more row groups than the grid and the workspace are for: then
+  // nothing is computed.
+  if (p.cu_q != nullptr && wave_sum_f(tokens) > (float)p.T) {
+    d.s.n = d.my_tiles = 0;
+    d.invalid = true;
+    return d;
   }
   int p_tiles = 0;
   if (p.P > 0) {
@@ -245,6 +255,7 @@ __device__ __forceinline__ Place find_place(const PagedParams& p, const Division
   const int c = (p.B + 63) >> 6;
   Place r{};
   r.b = -1;
+  if (d.invalid) return r;
   auto hits = [&](const Seq& s, int run_tiles, int run_units) {
     return __ballot(BY == kToken ? s.n > 0 && u < s.t0 + s.n : u < (BY == kWideUnit ? run_units : run_tiles));
   };

@@ -312,7 +312,6 @@ __device__ __forceinline__ void write_row(const PagedParams& p, const Unit& u, c
     if (p.lse != nullptr && quad == 0) p.lse[lse_at] = l == 0.f ? -INFINITY : (m + fast_log2(l)) * kLn2;
     return;
   }
-  if (u.slot >= (WIDE ? p.wide_slots : p.narrow_slots)) return;  // (only where cu_q descends)
   const int64_t at = ((int64_t)u.slot * p.Hkv + hk) * (WIDE ? p.wide_rows : p.narrow_rows) + rl;
   float* po = (WIDE ? p.wide_o : p.narrow_o) + at * D + 8 * quad;
   *reinterpret_cast<f32x4*>(po) = lo;
@@ -903,8 +902,6 @@ __global__ void __launch_bounds__(64 * kMergeWaves) paged_merge_kernel(PagedPara
     const int n_pre = d.p_ns > 0 ? d.p_ns : d.p_tiles > 0 ? (d.p_tiles - 1) / d.stretch + 1 : 0;
     const int n_all = n_pre + n_own;
     if (p.P == 0 && n_own == 1) continue;  // written by its unit
-    const int last_slot = own0 + (wide ? (row_groups(p, pl.s.n * p.G) - 1) * n_own : 0) + n_own - 1;
-    if (last_slot >= (wide ? p.wide_slots : p.narrow_slots)) return;  // (only where cu_q descends)
     const bool share = NG > 1 && (TEAM || n_all > 8 || r_to - r_from < NG);  // all groups on one row
     const int sub = (share ? grp : 0) + (TEAM ? w * NG : 0), step = (share ? NG : 1) * (TEAM ? kMergeWaves : 1);
     const int at_once = share ? 1 : NG;

@@ -38,6 +38,14 @@ def _device(*tensors):
     return index
 
 
+def _launch(dev: int, name: str, *args):
+    """The library call, with the tensors' device current (streams and kernels belong to one)."""
+    if torch.cuda.current_device() == dev:
+        return _lib.call(name, *args, _lib.stream_handle(dev))
+    with torch.cuda.device(dev):
+        return _lib.call(name, *args, _lib.stream_handle(dev))
+
+
 def _tokens(op: str, name: str, t: torch.Tensor, cu_q):
     """(batch, token, head) strides of a step's tokens."""
     st = t.stride()
@@ -127,9 +135,9 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, k_pages: torch.Tensor, 
     elif query_out is not None:
         raise RuntimeError(f"{op}: query_out without a query")
     strides = _STRIDES_19.pack(*q_st, *k_st, *v_st, *o_st, *pool_st, block_table.stride(0))
-    _lib.call("dgg_paged_append", q_ptr, key.data_ptr(), value.data_ptr(), o_ptr, k_pages.data_ptr(),
+    _launch(dev, "dgg_paged_append", q_ptr, key.data_ptr(), value.data_ptr(), o_ptr, k_pages.data_ptr(),
               v_pages.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), _lib.ptr(cu_q), B, T, Sq, Hq, Hkv, D,
-              n_pages, page, width, strides, rope_theta or 0.0, _lib.dtype_code(dtype), _lib.stream_handle(dev))
+              n_pages, page, width, strides, rope_theta or 0.0, _lib.dtype_code(dtype))
     return query_out
 
 
@@ -152,10 +160,10 @@ def _attend(op: str, q, k_pages, v_pages, block_table, kv_lens, prefix_len, cu_q
     ws = q.new_empty(ws_bytes // 2 + 8)  # (of 16-bit elements; another type is refused below)
     lse = torch.empty(T, Hq, dtype=torch.float32, device=q.device) if return_lse else None
     strides = _STRIDES_13.pack(*q_st, *pool_st, *o_st, block_table.stride(0))
-    _lib.call("dgg_attn_paged", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), _lib.ptr(lse),
+    _launch(dev, "dgg_attn_paged", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), _lib.ptr(lse),
               block_table.data_ptr(), kv_lens.data_ptr(), _lib.ptr(cu_q), ws.data_ptr(), ws_bytes, B, T, Sq, Hq, Hkv, D,
               n_pages, page, width, prefix_len, strides, 1.0 / math.sqrt(D) if scale is None else scale, softcap or 0.0,
-              window or 0, _lib.ATTN_CAUSAL if causal else 0, _lib.dtype_code(dtype), _lib.stream_handle(dev))
+              window or 0, _lib.ATTN_CAUSAL if causal else 0, _lib.dtype_code(dtype))
     if not return_lse:
         return out
     return out, lse if cu_q is not None else lse.view(B, Sq, Hq).transpose(1, 2)

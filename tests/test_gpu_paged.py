@@ -234,6 +234,21 @@ def test_holes_and_long_lengths(gpu):
     _check(out, lse, op.attention(q, kp, vp, table, [5000, 96]), "kv_len beyond the table")
 
 
+@pytest.mark.parametrize("prefix", [0, 16])
+def test_offsets_that_name_tokens_twice(gpu, prefix):
+    # a cu_q that descends: more tokens than the call has; nothing is computed
+    g = _gen(12)
+    kv = [40, 33, 64, 20]
+    kp, vp, table = _cache(g, kv, 16, 1, 64, torch.float16)
+    args = _to(gpu, kp, vp, table, kv)
+    q = torch.randn(48, 2, 64, generator=g).half().to(gpu)
+    cu = torch.tensor([0, 48, 0, 48, 10], dtype=torch.int32, device=gpu)
+    mark = torch.full_like(q, 7.0)
+    kw = dict(cu_q=cu, out=mark)
+    paged.shared_prefix_attention(q, *args, prefix, **kw) if prefix else paged.paged_attention(q, *args, **kw)
+    assert (mark == 7.0).all()
+
+
 def test_strided_inputs(gpu):
     # q as a slice of a projection, out with wider rows, a table that is part of a larger one
     g = _gen(8)
