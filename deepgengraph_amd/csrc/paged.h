@@ -1,10 +1,10 @@
-// Attention over a paged key/value cache: launch parameters and the division of the work, shared by the attention kernels
-// and the merge of paged_attention.hip.
+// Attention over a paged key/value cache: launch parameters and the division of the work, shared by the attention
+// kernels and the merge of paged_attention.hip.
 //
-// The batch is ragged: sequence b brings n_b query tokens (cu_q, or Sq each) and holds kv_b keys. The lengths are on the
-// device and the grid on the host, so every workgroup divides the work itself, from the same numbers with the same
-// arithmetic. All of it is per KV head; a sequence's n_b * G query rows that share the head are numbered token-major (row r
-// is token r / G, query head r % G), its keys are counted in tiles of 128.
+// The batch is ragged: sequence b brings n_b query tokens (cu_q, or Sq each) and holds kv_b keys. The lengths are on
+// the device and the grid on the host, so every workgroup divides the work itself, from the same numbers with the
+// same arithmetic. All of it is per KV head; a sequence's n_b * G query rows that share the head are numbered
+// token-major (row r is token r / G, query head r % G), its keys are counted in tiles of 128.
 //
 //   narrow  sequences of at most 32 rows. Their tiles, one sequence after the other, are cut into `narrow_wgs` equal
 //           stretches, one for each workgroup: a workgroup streams as many keys as any other, whatever the lengths are. A
@@ -68,8 +68,8 @@ void launch_d256(const PagedParams& p, bool bf16, hipStream_t st);
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// gi / gpp for gi < 2^26 (the quotient of a number of 32 bits by multiplication: gpp_mul = ceil(2^(32 + shift) / gpp) is
-// off by less than gpp * 2^-(32 + shift) of it, and shift is at least log2(gpp) - 6).
+// gi / gpp for gi < 2^26 (the quotient of a number of 32 bits by multiplication: gpp_mul = ceil(2^(32 + shift) / gpp)
+// is off by less than gpp * 2^-(32 + shift) of it, and shift is at least log2(gpp) - 6).
 __device__ __forceinline__ int page_index(const PagedParams& p, int gi) {
   return p.gpp == 1 ? gi : (int)(__umulhi((uint32_t)gi, p.gpp_mul) >> p.gpp_shift);
 }
@@ -100,7 +100,8 @@ __device__ __forceinline__ int first_key(const PagedParams& p, const Seq& s) {
 }
 __device__ __forceinline__ int key_tiles(int lo, int hi) { return hi > lo ? (hi + kTile - 1) / kTile - lo / kTile : 0; }
 
-// Sums, extremes and inclusive prefix sums over a wave, on the DPP lane shifts (a sixth of the latency of ds_bpermute).
+// Sums, extremes and inclusive prefix sums over a wave, on the DPP lane shifts (a sixth of the latency of
+// ds_bpermute).
 template <int CTRL, int ROWS>
 __device__ __forceinline__ int dpp_or(int old, int x) {
   return __builtin_amdgcn_update_dpp(old, x, CTRL, ROWS, 0xf, false);
@@ -132,8 +133,9 @@ __device__ __forceinline__ float wave_sum_f(float x) {
   })));
 }
 
-// What every wave finds out from all the lengths. Lane l looks at sequences l * c .. l * c + c - 1 (c = ceil(B / 64)); what
-// it found is kept, so that looking up a sequence later takes a ballot and not a second look at the lengths.
+// What every wave finds out from all the lengths. Lane l looks at sequences l * c .. l * c + c - 1 (c = ceil(B /
+// 64)); what it found is kept, so that looking up a sequence later takes a ballot and not a second look at the
+// lengths.
 struct Division {
   int slice;         // most key tiles of a wide unit
   int p_lo;          // first prefix key that any row sees
@@ -154,7 +156,8 @@ __device__ __forceinline__ int wide_slices(const PagedParams& p, const Seq& s, i
 }
 // Narrow tiles of a sequence, its wide units and their partial slots.
 template <bool WIDE>
-__device__ __forceinline__ void count_seq(const PagedParams& p, const Seq& s, int slice, int& tiles, int& units, int& slots) {
+__device__ __forceinline__ void count_seq(const PagedParams& p, const Seq& s, int slice, int& tiles, int& units,
+                                          int& slots) {
   tiles = units = slots = 0;
   if (s.n == 0) return;
   if (!is_wide(p, s)) {
@@ -187,8 +190,8 @@ __device__ __forceinline__ Division divide(const PagedParams& p, int lane) {
     }
     lo = min(lo, p.window > 0 ? max(0, d.s.kv - d.s.n - p.window + 1) : 0);
   }
-  // A cu_q that descends can name a token more than once, and more row groups than the grid and the workspace are for: then
-  // nothing is computed.
+  // A cu_q that descends can name a token more than once, and more row groups than the grid and the workspace are
+  // for: then nothing is computed.
   if (p.cu_q != nullptr && wave_sum_f(tokens) > (float)p.T) {
     d.s.n = d.my_tiles = 0;
     d.invalid = true;
@@ -214,9 +217,10 @@ __device__ __forceinline__ Division divide(const PagedParams& p, int lane) {
       work += (float)d.p_rg * (float)p_tiles;
       groups += (float)d.p_rg;
     }
-    // At least work / wide_target: the sum of 4096 terms in fp32 is off by less than 2^-12 of it. Where the row groups
-    // alone are three quarters of the units wanted, only those half as long again as the mean are cut (4 x 1,024 tokens
-    // over 4,096 keys, 16 heads of 64: 512 row groups, 672 wanted; 109 us with each cut in two, 98 without).
+    // At least work / wide_target: the sum of 4096 terms in fp32 is off by less than 2^-12 of it. Where the row
+    // groups alone are three quarters of the units wanted, only those half as long again as the mean are cut (4 x
+    // 1,024 tokens over 4,096 keys, 16 heads of 64: 512 row groups, 672 wanted; 109 us with each cut in two, 98
+    // without).
     const float per = work * p.per_wide;
     d.slice = max(1, (int)ceilf(min(groups * p.per_wide >= 0.75f ? 1.5f * per : per, 1e9f)));
     if (d.p_rg > 0) d.p_ns = ceil_div(p_tiles, d.slice);

@@ -4,12 +4,13 @@
 //   token i of sequence b sits at pos = kv_len[b] - n_b + i; angle_j = pos * theta^(-2j/D), pairs (j, j + D/2):
 //   k_page[pos % page] = (x cos - y sin, y cos + x sin), v_page[pos % page] = v, query likewise to its own output.
 //
-// Bound by the bytes of a large call (6,072 tokens of 32 + 32 + 32 heads, fp16, 299 MB read and written: 57 us in the kernel
-// trace, 5.3 TB/s, where a large copy reaches 4.8) and by the chain lengths -> page number -> store of a small one (64
-// tokens: 4 us). A workgroup takes a part of one token's heads: its data are requested before the token's position and page
-// are known, and the D/2 (cos, sin) pairs are computed once, in the LDS, for all heads. The angle is taken in 64 bits, as
-// turns (pos * theta^(-2j/D) / 2 pi, less its nearest whole number): in 32 bits a position of 100,000 would leave an error
-// of a hundredth of a radian. From there on 32 bits do: one rounding to the storage type at the end.
+// Bound by the bytes of a large call (6,072 tokens of 32 + 32 + 32 heads, fp16, 299 MB read and written: 57 us in the
+// kernel trace, 5.3 TB/s, where a large copy reaches 4.8) and by the chain lengths -> page number -> store of a small
+// one (64 tokens: 4 us). A workgroup takes a part of one token's heads: its data are requested before the token's
+// position and page are known, and the D/2 (cos, sin) pairs are computed once, in the LDS, for all heads. The angle
+// is taken in 64 bits, as turns (pos * theta^(-2j/D) / 2 pi, less its nearest whole number): in 32 bits a position of
+// 100,000 would leave an error of a hundredth of a radian. From there on 32 bits do: one rounding to the storage type
+// at the end.
 #include "common.h"
 
 namespace {
@@ -58,9 +59,9 @@ __device__ __forceinline__ void store8(typename T::scalar* p, f32x8 v) {
   }
 }
 
-// An item is 8 elements of each half of a head: the query heads' first, then the keys', then the values'. One for each thread:
-// more workgroups per token, which repeat the look-up and the angles, but shorter ones (64 tokens of 32 + 8 + 8 heads 4.0 us
-// against 4.6 with four, 4,096 of them 23.8 against 25.9).
+// An item is 8 elements of each half of a head: the query heads' first, then the keys', then the values'. One for
+// each thread: more workgroups per token, which repeat the look-up and the angles, but shorter ones (64 tokens of 32
+// + 8 + 8 heads 4.0 us against 4.6 with four, 4,096 of them 23.8 against 25.9).
 template <typename T, bool ROPE>
 __global__ void __launch_bounds__(kThreads) paged_append_kernel(AppendParams p) {
   typedef typename T::scalar S;

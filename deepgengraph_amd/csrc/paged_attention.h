@@ -6,8 +6,8 @@
 // in tiles of keys that go straight from the pages to the LDS (global_load_lds, DmaLayout of attention_common.h):
 //   S^T (32 keys x 32 rows) = K . Q^T     v_mfma_f32_32x32x16, A = K from the LDS, B = Q in registers
 //   O^T (D x 32 rows)      += V^T . P^T   A = V^T by transposing LDS reads, B = P from the S^T accumulator
-// with one running maximum and sum per row, in fp32; P is rounded to the storage type, as the matrix instruction takes it
-// (its error is that of the output's own rounding, spread over the keys). Two ways:
+// with one running maximum and sum per row, in fp32; P is rounded to the storage type, as the matrix instruction
+// takes it (its error is that of the output's own rounding, spread over the keys). Two ways:
 //   narrow  up to 32 rows of a KV head: bound by the stream of keys and values. The waves share the rows and take the
 //           32-key tiles in turn, each with buffers of its own and no barrier, and add their states at the end;
 //   wide    more rows: bound by the matrix products. The waves share the tiles and have rows of their own.
@@ -30,8 +30,8 @@ namespace {
 using namespace dgg_attn;
 using namespace dgg_paged;
 
-// The launch parameters, read from the kernel's arguments anew: a part of the kernel that begins with this does not keep
-// scalar registers for what other parts use (without it 80 to 150 of them spill).
+// The launch parameters, read from the kernel's arguments anew: a part of the kernel that begins with this does not
+// keep scalar registers for what other parts use (without it 80 to 150 of them spill).
 __device__ __forceinline__ const PagedParams& fresh_params() {
   auto at = (const PagedParams __attribute__((address_space(4)))*)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(at));
@@ -127,8 +127,8 @@ __device__ __forceinline__ Seen seen_by_wave(const PagedParams& p, const Unit& u
   return v;
 }
 
-// The pages of 64 granules, one per lane, and which of the granules hold a key of the unit. The page numbers of the next 64
-// are requested when these are taken up, so that their latency is not waited for.
+// The pages of 64 granules, one per lane, and which of the granules hold a key of the unit. The page numbers of the
+// next 64 are requested when these are taken up, so that their latency is not waited for.
 struct Granules {
   const int32_t* row;  // the sequence's row of the table
   int page, next;
@@ -161,8 +161,8 @@ __device__ __forceinline__ void copy16(uint32_t lds, const void* sbase, uint32_t
     dma16(lds, sbase, voff);
 }
 
-// Copies one granule (16 rows of D) of K or V to `lds`, the place of its first 4- or 8-row group. kWhole: every row is a
-// key. Otherwise rows outside [first, last] are replaced by the nearest that is inside.
+// Copies one granule (16 rows of D) of K or V to `lds`, the place of its first 4- or 8-row group. kWhole: every row
+// is a key. Otherwise rows outside [first, last] are replaced by the nearest that is inside.
 template <int D, bool NT>
 struct GranuleCopy {
   typedef DmaLayout<D> L;
@@ -267,8 +267,8 @@ struct State {
 
 constexpr int kOQ = 64 * 16 + 16;  // a quad of O registers of a wave in the LDS, and padding
 
-// Leaves a wave's state in its slot: D / 8 quads of O, and (maximum in the exp2 domain, sum) of each row. ok: the lane has
-// a row (lanes without one would take their turns at the LDS, too).
+// Leaves a wave's state in its slot: D / 8 quads of O, and (maximum in the exp2 domain, sum) of each row. ok: the
+// lane has a row (lanes without one would take their turns at the LDS, too).
 template <int D>
 __device__ __forceinline__ void put_state(const State<D>& st, char* slot, f32x2* ml, float c, int lane, bool ok) {
   const float l = half_swap_sum(st.l[0] + st.l[1]);
@@ -282,7 +282,8 @@ __device__ __forceinline__ void put_state(const State<D>& st, char* slot, f32x2*
   if (lane < 32) ml[lane] = f32x2{st.m == -INFINITY ? -INFINITY : st.m * c, l};
 }
 
-// Joins KG states (slot i * step) of a row and writes 8 of its head-dim elements: the output, or a partial of the unit.
+// Joins KG states (slot i * step) of a row and writes 8 of its head-dim elements: the output, or a partial of the
+// unit.
 template <typename T, int D, int KG, bool WIDE>
 __device__ __forceinline__ void write_row(const PagedParams& p, const Unit& u, const char* slots, const f32x2* ml, int step,
                                           int slot_b, int r, int quad, int64_t o_off, int lse_at, int rl, int hk) {
@@ -336,8 +337,8 @@ __device__ __forceinline__ float block_scores(f32x16& s, const PagedParams& p, i
   return mloc;
 }
 
-// LDS of the two ways: NW waves' K and V buffers (which their O takes afterwards) and row states; two stages of a tile of
-// 16 keys per wave.
+// LDS of the two ways: NW waves' K and V buffers (which their O takes afterwards) and row states; two stages of a
+// tile of 16 keys per wave.
 template <int D, int NW>
 struct Lds {
   typedef DmaLayout<D> L;
@@ -372,6 +373,14 @@ struct NarrowTiles {
 };
 
 // One narrow unit: its keys over NW waves. page: first_page(); ahead(): called when the first copies are on their way.
+//
+// Bound by the stream of keys and values: per 32-key tile a wave moves 16 KiB (head_dim 128) and runs 16 MFMAs, about
+// a tenth of the time that its share of the memory takes. A wave has one K and one V buffer: K of the next tile is
+// requested as soon as this one's products have read it, V likewise, so that nearly all of its 16 KiB is always in
+// flight, with no barrier and no registers for it. The copies are non-temporal (each row is read once): 64 sequences
+// of 7,000 keys, 32 / 8 heads, 317 us without the hint, 289 with. Measured on MI355X: 64 sequences of 512 to 32,768
+// keys, fp16, 1.83 GB, 293 us (6.3 TB/s; the contiguous kernels reach 6.6 to 6.85 on caches of one length), 16
+// sequences of 32 heads, 1.70 GB, 266 us (6.4).
 template <typename T, int D, int NW, bool SOFTCAP, typename F>
 __device__ __forceinline__ void narrow_unit(const Unit& u, char* smem, int hk, int page, F&& ahead) {
   typedef typename T::scalar S;
@@ -545,8 +554,8 @@ __device__ __forceinline__ int narrow_segment(const PagedParams& p, const Divisi
   return last;
 }
 
-// The stretch of narrow workgroup `wg`, segment by segment. The first page numbers of the next segment are requested while
-// the present one streams: behind its 32 MB in flight a load takes 5 us.
+// The stretch of narrow workgroup `wg`, segment by segment. The first page numbers of the next segment are requested
+// while the present one streams: behind its 32 MB in flight a load takes 5 us.
 template <typename T, int D, int NW, bool WIDE, bool SOFTCAP>
 __device__ __forceinline__ void narrow_stretch(const Division& d, char* smem, int hk, int wg) {
   const int from = wg * d.stretch, to = min(d.tiles, from + d.stretch);
@@ -588,7 +597,9 @@ __device__ __forceinline__ bool wide_unit_of(const PagedParams& p, const Divisio
     const int nrg = row_groups(p, pl.s.n * p.G);
     ns = wide_slices(p, pl.s, d.slice);
     k = pl.local / nrg;
-    const int rg = nrg - 1 - (pl.local - k * nrg);  // under a causal mask the last row group sees the most keys: it goes first
+    // Under a causal mask the last row groups see the most keys: they go first (a prompt of 4,096 tokens 180 -> 150
+    // us).
+    const int rg = nrg - 1 - (pl.local - k * nrg);
     u.b = pl.b;
     u.s = pl.s;
     u.row0 = rg * R;
@@ -603,7 +614,14 @@ __device__ __forceinline__ bool wide_unit_of(const PagedParams& p, const Divisio
 }
 
 // One wide unit: NW waves over tiles of BN keys in a ring of two. KG: waves that share the same 32 rows, each taking
-// BN / KG keys of every tile; a workgroup covers 32 * NW / KG rows. Each wave copies one granule of a tile (BN = 16 NW).
+// BN / KG keys of every tile; a workgroup covers 32 * NW / KG rows. Each wave copies one granule of a tile (BN = 16
+// NW).
+//
+// Bound by the matrix products and the LDS that feeds them, as the prefill forward, whose tiles, layout and order of
+// copies these are. Measured on MI355X: 4 x 1,024 tokens over 8,192 keys, bf16, 32 / 8 heads 491 us, 1,050 TFLOP/s,
+// beside 462 of that forward with an lse over a contiguous cache on the same box; where the 6% go was not found
+// (looking up the next tile's pages among the MFMAs changed nothing). Full and masked tiles have loops of their own:
+// one loop for both copied O from one's registers to the other's in every tile, 505 us against 476.
 template <typename T, int D, int NW, int KG, int OCC, bool SOFTCAP>
 __device__ __forceinline__ void wide_unit(const Unit& u, char* smem, int hk) {
   typedef DmaLayout<D> L;
@@ -697,8 +715,8 @@ __device__ __forceinline__ void wide_unit(const Unit& u, char* smem, int hk) {
     else asm volatile("" : "+v"(qf[kk]));
   }
 
-  // One tile. Full tiles issue the next tile's copies one by one among their QK^T steps, so that the issue overlaps the
-  // MFMAs instead of following the barrier as one burst.
+  // One tile. Full tiles issue the next tile's copies one by one among their QK^T steps, so that the issue overlaps
+  // the MFMAs instead of following the barrier as one burst.
   constexpr int CPS = (2 * LOADS + D / 16 - 1) / (D / 16);  // copies per QK^T step
   auto tile = [&](const int t, const unsigned holes, auto masked) {
     constexpr bool MASKED = decltype(masked)::value;
@@ -784,8 +802,8 @@ __device__ __forceinline__ void wide_unit(const Unit& u, char* smem, int hk) {
     }
   };
 
-  // Runs of full tiles and of others, in loops of their own (one loop with both would copy O from one's registers to the
-  // other's in every tile). look: the kind of tile t, and the granule copied during it.
+  // Runs of full tiles and of others, in loops of their own (one loop with both would copy O from one's registers to
+  // the other's in every tile). look: the kind of tile t, and the granule copied during it.
   unsigned holes = 0;
   bool more = false, full = false;
   auto look = [&](int t) __attribute__((always_inline)) {
@@ -862,11 +880,11 @@ paged_mixed_kernel(PagedParams p) {
   if (wide_unit_of(p, d, n - p.narrow_wgs, u)) wide_unit<T, D, NW, KG, OCC, SOFTCAP>(u, smem, hk);
 }
 
-// Joins the partials of rows: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, lse = (M + log2 L) ln 2, with those of the
-// prefix first and then the sequence's own. A wave takes rows_per_merge rows of the batch (token-major, as the prefix numbers
-// them) of a KV head, by itself: its time is the chain lengths -> partials -> output, once for each sequence that its rows
-// touch. Its groups of D / 4 lanes (four head-dim elements each) take rows in turn, or share one of many partials. TEAM: the
-// four waves of a workgroup share one row, where there are few.
+// Joins the partials of rows: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, lse = (M + log2 L) ln 2, with those
+// of the prefix first and then the sequence's own. A wave takes rows_per_merge rows of the batch (token-major, as the
+// prefix numbers them) of a KV head, by itself: its time is the chain lengths -> partials -> output, once for each
+// sequence that its rows touch. Its groups of D / 4 lanes (four head-dim elements each) take rows in turn, or share
+// one of many partials. TEAM: the four waves of a workgroup share one row, where there are few.
 constexpr int kMergeWaves = 4;
 template <typename T, int D, bool WIDE, bool TEAM>
 __global__ void __launch_bounds__(64 * kMergeWaves) paged_merge_kernel(PagedParams p) {
@@ -1025,8 +1043,8 @@ void launch_paged(const PagedParams& p, hipStream_t st) {
   else launch_cap<T, D, false>(p, st);
   const int64_t rows = (int64_t)p.T * p.G;
   const int64_t waves = (rows + p.rows_per_merge - 1) / p.rows_per_merge * p.Hkv;
-  // A workgroup per row up to 512 rows: two per CU (8 sequences of one token behind a prefix of 8,192, 256 rows of up to 66
-  // partials: 22.5 us against 25.4 with a wave for each; 64 sequences, 2,048 rows: 297 against 293).
+  // A workgroup per row up to 512 rows: two per CU (8 sequences of one token behind a prefix of 8,192, 256 rows of up
+  // to 66 partials: 22.5 us against 25.4 with a wave for each; 64 sequences, 2,048 rows: 297 against 293).
   const bool team = rows * p.Hkv <= 512;
   const dim3 grid((unsigned)(team ? waves : (waves + kMergeWaves - 1) / kMergeWaves)), block(64 * kMergeWaves);
   if (p.wide_units > 0) {

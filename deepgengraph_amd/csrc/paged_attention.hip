@@ -15,19 +15,18 @@ struct HostPlan {
     return ((int64_t)wide_slots * wide_rows + (int64_t)narrow_slots * narrow_rows) * Hkv * (D + 2);
   }
 };
-// Row groups. 64 rows (waves in pairs over the same rows) where there are no more; otherwise 128 rows, two workgroups of
-// four waves per CU, so that one streams or computes while the other begins or ends; but at head_dim 128 256 rows, one
-// workgroup of eight waves, for chunks that fill the chip with them: half the keys and values through the LDS. Measured on
-// MI355X, bf16, 32 / 8 heads, 128 / 256 rows, us: 2 x 1,024 tokens, 8,192 keys 272 / 245; 16 x 128, 2,048 92 / 83; 8 x 512,
-// 512 55 / 52; 4 x 128, 4,096 57.5 / 57.7; 262 tokens of 16 sequences behind a prefix of 16,384 104 / 122; a step of 28
-// decode rows and 4 chunks 137 / 146.
-// Units wanted: as many as are resident at once or a little fewer, for the row groups' last slices are short (the same
-// step at 256, 384, 448, 512 units 138, 136, 135, 131; 8 chunks of up to 1,024 tokens 148, 147, 147, 158; the prefix of
-// 16,384 133, 106, 101, 100).
-// Narrow stretches: one for each resident workgroup, of at most two per CU (32 x 16 heads of 64, up to 4,000 keys: 512
-// stretches 53, 768 56). Beside wide units one per CU: that many saturate the memory, and more only lengthen the latency
-// that the wide units see (the step of 28 decode rows and 4 chunks at 128, 256, 384 stretches 129, 127, 132, 64 decode rows
-// behind a prefix of 8,192 77, 55, 55).
+// Row groups. 64 rows (waves in pairs over the same rows) where there are no more; otherwise 128 rows, two workgroups
+// of four waves per CU, so that one streams or computes while the other begins or ends; but at head_dim 128 256 rows,
+// one workgroup of eight waves, for chunks that fill the chip with them: half the keys and values through the LDS.
+// Measured on MI355X, bf16, 32 / 8 heads, 128 / 256 rows, us: 2 x 1,024 tokens, 8,192 keys 272 / 245; 16 x 128, 2,048
+// 92 / 83; 8 x 512, 512 55 / 52; 4 x 128, 4,096 57.5 / 57.7; 262 tokens of 16 sequences behind a prefix of 16,384 104
+// / 122; a step of 28 decode rows and 4 chunks 137 / 146. Units wanted: as many as are resident at once or a little
+// fewer, for the row groups' last slices are short (the same step at 256, 384, 448, 512 units 138, 136, 135, 131; 8
+// chunks of up to 1,024 tokens 148, 147, 147, 158; the prefix of 16,384 133, 106, 101, 100). Narrow stretches: one
+// for each resident workgroup, of at most two per CU (32 x 16 heads of 64, up to 4,000 keys: 512 stretches 53, 768
+// 56). Beside wide units one per CU: that many saturate the memory, and more only lengthen the latency that the wide
+// units see (the step of 28 decode rows and 4 chunks at 128, 256, 384 stretches 129, 127, 132, 64 decode rows behind
+// a prefix of 8,192 77, 55, 55).
 HostPlan host_plan(int64_t B, int64_t T, bool ragged, int64_t Hq, int64_t Hkv, int64_t D, int64_t P) {
   HostPlan h{};
   const int64_t G = Hq / Hkv, Sq = T / B, CUs = 256;
@@ -51,7 +50,8 @@ HostPlan host_plan(int64_t B, int64_t T, bool ragged, int64_t Hq, int64_t Hkv, i
     h.wide_rows = (int)std::min<int64_t>(R, h.prefix_wide ? T * G : most);
   }
   if (narrow) {
-    h.narrow_wgs = (int)std::max<int64_t>(1, (wide ? std::min(CUs, CUs * per_cu * 3 / 4) : CUs * std::min<int64_t>(per_cu, 2)) / Hkv);
+    const int64_t wgs = wide ? std::min(CUs, CUs * per_cu * 3 / 4) : CUs * std::min<int64_t>(per_cu, 2);
+    h.narrow_wgs = (int)std::max<int64_t>(1, wgs / Hkv);
     h.narrow_slots = (int)(h.narrow_wgs + B + 1);
     h.narrow_rows = (int)std::min<int64_t>(dgg_paged::kNarrowRows, P > 0 && !h.prefix_wide ? T * G : most);
   }
@@ -146,7 +146,8 @@ extern "C" int dgg_attn_paged(const void* q, const void* k_pages, const void* v_
     ws += n;
     return at;
   };
-  const int64_t wide_all = (int64_t)h.wide_slots * h.wide_rows * Hkv, narrow_all = (int64_t)h.narrow_slots * h.narrow_rows * Hkv;
+  const int64_t wide_all = (int64_t)h.wide_slots * h.wide_rows * Hkv;
+  const int64_t narrow_all = (int64_t)h.narrow_slots * h.narrow_rows * Hkv;
   p.wide_o = carve(wide_all * D);
   p.narrow_o = carve(narrow_all * D);
   p.wide_ml = carve(wide_all * 2);

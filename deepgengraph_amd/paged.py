@@ -24,6 +24,7 @@ import torch
 from . import _lib
 
 _I32 = torch.int32
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _STRIDES_19, _STRIDES_13 = struct.Struct("19q"), struct.Struct("13q")
 
 
@@ -40,7 +41,7 @@ def _device(*tensors):
 
 def _launch(dev: int, name: str, *args):
     """The library call, with the tensors' device current (streams and kernels belong to one)."""
-    if torch.cuda.current_device() == dev:
+    if _current_device() == dev:
         return _lib.call(name, *args, _lib.stream_handle(dev))
     with torch.cuda.device(dev):
         return _lib.call(name, *args, _lib.stream_handle(dev))

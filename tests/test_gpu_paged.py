@@ -501,7 +501,8 @@ def test_step_together_captured(gpu):
     def step(qkv, kd, vd, td, ld):
         q, k, v = (x.unflatten(-1, (-1, D)) for x in qkv.split([Hq * D, Hkv * D, Hkv * D], dim=-1))
         q = paged.paged_append(k, v, kd, vd, td, ld, query=q, rope_theta=1e4)
-        return paged.paged_attention(q, kd, vd, td, ld, return_lse=True), paged.shared_prefix_attention(q, kd, vd, td, ld, 32)
+        return (paged.paged_attention(q, kd, vd, td, ld, return_lse=True),
+                paged.shared_prefix_attention(q, kd, vd, td, ld, 32))
 
     kd, vd, td = kp0.to(gpu), vp0.to(gpu), table.to(gpu)
     ld = torch.tensor([40, 33, 50], dtype=torch.int32, device=gpu)
