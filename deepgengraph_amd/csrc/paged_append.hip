@@ -161,8 +161,8 @@ extern "C" int dgg_paged_append(const void* q, const void* k, const void* v, voi
   DGG_REQUIRE(dgg::valid_dtype(dtype), DGG_ERR_DTYPE, "%s: unsupported dtype code %d", op, dtype);
   DGG_REQUIRE(B >= 0 && B <= (1 << 20) && T >= 0 && T < (1 << 24), DGG_ERR_SHAPE,
               "%s: bad sizes (B=%lld of at most 2^20, %lld tokens of fewer than 2^24)", op, (long long)B, (long long)T);
-  DGG_REQUIRE(Sq >= 0 && (Sq == 0 || Sq * B == T), DGG_ERR_SHAPE, "%s: %lld tokens are not %lld sequences of %lld", op,
-              (long long)T, (long long)B, (long long)Sq);
+  DGG_REQUIRE(Sq >= 0 && Sq < (1 << 24) && (Sq == 0 || Sq * B == T), DGG_ERR_SHAPE,
+              "%s: %lld tokens are not %lld sequences of %lld", op, (long long)T, (long long)B, (long long)Sq);
   DGG_REQUIRE((cu_q == nullptr) == (Sq > 0) || T == 0, DGG_ERR_SHAPE,
               "%s: give cu_q, or Sq tokens for every sequence, and not both", op);
   DGG_REQUIRE(Hq >= 0 && Hq <= 1024 && Hkv > 0 && Hkv <= 1024, DGG_ERR_SHAPE, "%s: bad head counts %lld / %lld", op,
@@ -173,7 +173,7 @@ extern "C" int dgg_paged_append(const void* q, const void* k, const void* v, voi
               (long long)num_pages);
   DGG_REQUIRE(page_size > 0 && page_size <= (1 << 20), DGG_ERR_SHAPE, "%s: page_size %lld must be in [1, 2^20]", op,
               (long long)page_size);
-  DGG_REQUIRE(table_width >= 0 && table_width * page_size < (1ll << 31), DGG_ERR_SHAPE,
+  DGG_REQUIRE(table_width >= 0 && table_width < (1ll << 31) && table_width * page_size < (1ll << 31), DGG_ERR_SHAPE,
               "%s: a block table row of %lld pages of %lld is too long", op, (long long)table_width,
               (long long)page_size);
   DGG_REQUIRE(rope_theta == 0.f || (std::isfinite(rope_theta) && rope_theta > 0.f), DGG_ERR_SHAPE,

@@ -61,8 +61,8 @@ HostPlan host_plan(int64_t B, int64_t T, bool ragged, int64_t Hq, int64_t Hkv, i
 int check_sizes(const char* op, int64_t B, int64_t T, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix) {
   DGG_REQUIRE(B >= 0 && B <= 4096 && T >= 0 && T < (1 << 24), DGG_ERR_SHAPE,
               "%s: bad sizes (B=%lld of at most 4096, %lld tokens of fewer than 2^24)", op, (long long)B, (long long)T);
-  DGG_REQUIRE(Sq >= 0 && (Sq == 0 || Sq * B == T), DGG_ERR_SHAPE, "%s: %lld tokens are not %lld sequences of %lld", op,
-              (long long)T, (long long)B, (long long)Sq);
+  DGG_REQUIRE(Sq >= 0 && Sq < (1 << 24) && (Sq == 0 || Sq * B == T), DGG_ERR_SHAPE,
+              "%s: %lld tokens are not %lld sequences of %lld", op, (long long)T, (long long)B, (long long)Sq);
   DGG_REQUIRE(Hq > 0 && Hkv > 0 && Hq <= 1024 && Hq % Hkv == 0, DGG_ERR_SHAPE, "%s: bad head counts (Hq=%lld Hkv=%lld)",
               op, (long long)Hq, (long long)Hkv);
   DGG_REQUIRE(T * Hq < (1 << 28), DGG_ERR_SHAPE, "%s: too many query rows (%lld tokens of %lld heads)", op, (long long)T,
@@ -99,7 +99,7 @@ extern "C" int dgg_attn_paged(const void* q, const void* k_pages, const void* v_
   DGG_REQUIRE(page_size > 0 && page_size % dgg_paged::kGranule == 0 && page_size <= (1 << 20), DGG_ERR_SHAPE,
               "%s: page_size %lld must be a multiple of %d of at most 2^20", op, (long long)page_size,
               dgg_paged::kGranule);
-  DGG_REQUIRE(table_width >= 0 && table_width * page_size < (1ll << 30), DGG_ERR_SHAPE,
+  DGG_REQUIRE(table_width >= 0 && table_width < (1ll << 30) && table_width * page_size < (1ll << 30), DGG_ERR_SHAPE,
               "%s: a block table row of %lld pages of %lld is too long", op, (long long)table_width,
               (long long)page_size);
   DGG_REQUIRE(B * table_width * page_size < (1ll << 37), DGG_ERR_SHAPE, "%s: a block table of more than 2^37 keys", op);

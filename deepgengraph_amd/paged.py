@@ -182,7 +182,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     float16 and bfloat16, D 64, 128 or 256, page sizes that are multiples of 16, up to 4,096 sequences. A kv_lens beyond
     the table's row is taken as what that row can name, and keys on a page number outside the pool are not seen (a window's
     pages may be given back by writing -1 into the table). A row that sees no key gets 0 and lse -inf; rows from cu_q[B]
-    on are not written. Memory behind a sequence's last key may hold anything, NaN included."""
+    on are not written. out may be q itself. Memory behind a sequence's last key may hold anything, NaN included."""
     return _attend("paged_attention", q, k_pages, v_pages, block_table, kv_lens, 0, cu_q, causal, softcap, window, scale,
                    return_lse, out)
 

@@ -490,6 +490,72 @@ def test_llama_block_over_a_paged_cache(gpu, prefix):
         _check(y.unflatten(-1, (H, D)), None, ref, f"step {n}")
 
 
+@pytest.mark.parametrize("prefix", [0, 48])
+@pytest.mark.parametrize("n,kv", [([1, 1, 1], [300, 60, 2000]), ([1, 150, 9], [300, 160, 2000]), ([70, 70], [500, 80])])
+def test_output_over_the_query(gpu, n, kv, prefix):
+    """The output may take the query's place: one unit, cut keys and a shared prefix give what they give elsewhere."""
+    g = _gen(41)
+    kp, vp, table = _cache(g, kv, 16, 2, 128, torch.bfloat16, shared=prefix)
+    args = _to(gpu, kp, vp, table, kv)
+    same = len(set(n)) == 1
+    cu = None if same else torch.tensor([0, *torch.tensor(n).cumsum(0).tolist()], dtype=torch.int32, device=gpu)
+    q = torch.randn(*((len(n), n[0]) if same else (sum(n),)), 8, 128, generator=g).bfloat16().to(gpu)
+    call = dict(cu_q=cu)
+    f = paged.paged_attention if not prefix else lambda *a, **k: paged.shared_prefix_attention(*a, prefix, **k)
+    want = f(q, *args, **call)
+    assert f(q, *args, out=q, **call) is q
+    assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_ragged_batch_captured(gpu, D):
+    """A batch of fixed capacity, captured once and replayed with other numbers of tokens per sequence: decode rows, chunks,
+    sequences without tokens, all rows or few of them in use. Every replay against the eager calls and the oracle; rows
+    behind the last sequence stay as they are."""
+    g = _gen(43)
+    B, T, Hq, Hkv, page, width, P = 5, 160, 8, 2, 16, 40, 32
+    table = torch.randperm(B * width, generator=g).view(B, width).to(torch.int32)
+    table[1:, : P // page] = table[0, : P // page]
+    kp, vp = (torch.randn(B * width, page, Hkv, D, generator=g).bfloat16() for _ in range(2))
+    kd, vd, td = kp.to(gpu), vp.to(gpu), table.to(gpu)
+    ld = torch.full((B,), 100, dtype=torch.int32, device=gpu)
+    cu = torch.zeros(B + 1, dtype=torch.int32, device=gpu)
+    q = torch.randn(T, Hq, D, generator=g).bfloat16().to(gpu)
+    outs = [torch.zeros_like(q) for _ in range(2)]
+
+    def step(o1, o2):
+        return (paged.paged_attention(q, kd, vd, td, ld, cu_q=cu, return_lse=True, out=o1)[1],
+                paged.shared_prefix_attention(q, kd, vd, td, ld, P, cu_q=cu, return_lse=True, out=o2)[1])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*outs)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lses = step(*outs)
+    for r, (n, kv) in enumerate([([1, 1, 1, 1, 1], [640, 33, 200, 1, 90]), ([1, 150, 0, 8, 1], [300, 182, 77, 600, 0]),
+                                 ([0, 0, 0, 0, 0], [50, 50, 50, 50, 50]), ([0, 0, 160, 0, 0], [40, 0, 640, 40, 40]),
+                                 ([9, 1, 33, 70, 4], [41, 1, 65, 102, 640])]):
+        cu.copy_(torch.tensor([0, *torch.tensor(n).cumsum(0).tolist()], dtype=torch.int32))
+        ld.copy_(torch.tensor(kv, dtype=torch.int32))
+        q.copy_(torch.randn(q.shape, generator=g).bfloat16())
+        for o in outs:
+            o.fill_(7.0)
+        graph.replay()
+        eager = [torch.full_like(q, 7.0) for _ in range(2)]
+        el = step(*eager)
+        torch.cuda.synchronize()
+        live = sum(n)
+        want = op.attention(q.cpu(), kp, vp, table, kv, cu_q=cu.cpu())
+        for i in range(2):
+            assert torch.equal(outs[i], eager[i]), f"replay {r}: output {i}"
+            assert torch.equal(lses[i][:live], el[i][:live]), f"replay {r}: lse {i}"
+            assert (outs[i][live:] == 7.0).all(), f"replay {r}: rows behind the last sequence"
+            _check(outs[i], lses[i], want, f"replay {r}, form {i}")
+
+
 def test_step_together_captured(gpu):
     """Append and attention as a decode step, captured once and replayed with other lengths, tables and inputs, against the
     eager calls; another stream in between."""

@@ -111,6 +111,15 @@ def test_append_refusals(lib):
     assert _append(lib, B=0, T=0, q=None) == OK
 
 
+def test_sizes_whose_products_pass_64_bits(lib):
+    # the products of the checks wrap around to sizes that would be right
+    for f in (_attn, _append):
+        assert f(lib, B=4096, T=4096, Sq=(1 << 52) + 1) == E_SHAPE
+        assert f(lib, width=1 << 60) == E_SHAPE
+        assert f(lib, width=(1 << 60) + 4) == E_SHAPE
+    assert lib.dgg_attn_paged_workspace_bytes(4096, 4096, (1 << 52) + 1, 4, 2, 128, 0) == -1
+
+
 def test_oracle_against_the_contiguous_one():
     """The paged oracle over pages in order is the contiguous oracle's attention of each sequence."""
     g = torch.Generator().manual_seed(0)
