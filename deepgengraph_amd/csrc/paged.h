@@ -6,8 +6,8 @@
 // same arithmetic. All of it is per KV head; a sequence's n_b * G query rows that share the head are numbered
 // token-major (row r is token r / G, query head r % G), its keys are counted in tiles of 128.
 //
-//   narrow  sequences of at most 32 rows. Their tiles, one sequence after the other, are cut into `narrow_wgs` equal
-//           stretches, one for each workgroup: a workgroup streams as many keys as any other, whatever the lengths are. A
+//   narrow  sequences of at most 32 rows. Their tiles, one sequence after the other, are cut into equal stretches,
+//           one for each workgroup: a workgroup streams as many keys as any other, whatever the lengths are. A
 //           stretch's part of a sequence is a segment; segment (workgroup i, sequence b) leaves its partial in slot i + b.
 //   wide    sequences of more rows, in row groups of R. The keys a row group sees are cut into ns_b slices, so that a unit
 //           (row group, slice) is at most `slice` tiles long: the tiles of all units over the units wanted (wide_target).
@@ -54,9 +54,10 @@ struct PagedParams {
   int log2_r;               // row group of wide units
   int prefix_wide;          // the prefix's rows are more than 32
   int wide_units, wide_slots, wide_rows;  // units in the grid; partial slots, and rows of one
-  int narrow_wgs, narrow_slots, narrow_rows;
+  int narrow_wgs, narrow_most, narrow_slots, narrow_rows;  // workgroups among wide sequences, and at most
   int rows_per_merge;
-  float per_wide;           // (1 + 2^-11) / wide_target
+  int places;               // workgroups that are resident at once
+  int wide_target;          // wide units wanted, at most
   dgg_attn::AttnParams s;   // scale and soft-cap constants (score_value)
 };
 
@@ -141,7 +142,8 @@ struct Division {
   int p_lo;          // first prefix key that any row sees
   int p_rg, p_ns;    // wide prefix: row groups and slices
   int p_tiles;       // narrow prefix: tiles
-  int stretch;       // tiles of a narrow workgroup
+  int narrow;        // workgroups with narrow stretches
+  int stretch;       // tiles of one
   int tiles;         // all narrow tiles
   bool invalid;      // the lengths make no sense
   // per lane: the last of its sequences, and its own and the running number of narrow tiles, wide units, partial slots
@@ -186,7 +188,7 @@ __device__ __forceinline__ Division divide(const PagedParams& p, int lane) {
     else if (WIDE) {
       const float nrg = (float)row_groups(p, d.s.n * p.G);
       groups += nrg;
-      work += nrg * (float)seq_tiles(p, d.s);
+      work = fmaf(nrg, (float)seq_tiles(p, d.s), work);
     }
     lo = min(lo, p.window > 0 ? max(0, d.s.kv - d.s.n - p.window + 1) : 0);
   }
@@ -208,21 +210,35 @@ __device__ __forceinline__ Division divide(const PagedParams& p, int lane) {
     d.p_tiles = p_tiles;
     d.tiles += p_tiles;
   }
-  d.stretch = p.narrow_wgs > 0 ? ceil_div(d.tiles, p.narrow_wgs) : 0;
+  d.narrow = p.narrow_wgs;
   if constexpr (WIDE) {
     work = wave_sum_f(work);
     groups = wave_sum_f(groups);
+    int units = p.wide_target;
+    const bool only_prefix = groups == 0.f;  // no sequence is wide
     if (p.prefix_wide) {
       d.p_rg = row_groups(p, p.T * p.G);
-      work += (float)d.p_rg * (float)p_tiles;
+      work = fmaf((float)d.p_rg, (float)p_tiles, work);
       groups += (float)d.p_rg;
     }
+    // Then stretches and the prefix's units share the places by their tiles, so that everything is resident at once
+    // and ends at about the same time. Measured on MI355X with the fixed numbers of host_plan / this, us: 64 decode
+    // rows behind 8,192 keys, 32 / 8 heads of 128, 56 / 50, 16 heads of 64 62 / 48; 32 rows, 16 / 8 heads of 256, 57 /
+    // 45; 64 x 1 or 2 tokens over up to 4,096 keys and no prefix, 16 heads of 64, 123 / 93. Among wide sequences,
+    // whose last row groups and slices are uneven, the same rule gains and loses (a step of 28 decode rows and 4
+    // chunks 132 / 135, 27 and 5 of head_dim 256 140 / 148, 8 chunks of up to 256 tokens 43 / 39).
+    if (only_prefix && d.tiles > 0) {
+      const float part = (float)d.tiles / ((float)d.tiles + work);
+      d.narrow = clampi((int)rintf((float)p.places * part), 1, min(p.places - 1, p.narrow_most));
+      units = min(p.places - d.narrow, p.wide_target);
+    }
+    const float per_unit = (1.0f + 1.0f / 2048) / (float)units;
     // At least work / wide_target: the sum of 4096 terms in fp32 is off by less than 2^-12 of it. Where the row
     // groups alone are three quarters of the units wanted, only those half as long again as the mean are cut (4 x
     // 1,024 tokens over 4,096 keys, 16 heads of 64: 512 row groups, 672 wanted; 109 us with each cut in two, 98
     // without).
-    const float per = work * p.per_wide;
-    d.slice = max(1, (int)ceilf(min(groups * p.per_wide >= 0.75f ? 1.5f * per : per, 1e9f)));
+    const float per = work * per_unit;
+    d.slice = max(1, (int)ceilf(min(groups * per_unit >= 0.75f ? 1.5f * per : per, 1e9f)));
     if (d.p_rg > 0) d.p_ns = ceil_div(p_tiles, d.slice);
     if (c == 1) {
       if (lane < p.B) {
@@ -240,6 +256,7 @@ __device__ __forceinline__ Division divide(const PagedParams& p, int lane) {
     d.run_units = wave_scan_add(d.my_units);
     d.run_slots = wave_scan_add(d.my_slots);
   }
+  d.stretch = d.narrow > 0 ? ceil_div(d.tiles, d.narrow) : 0;
   return d;
 }
 

@@ -872,12 +872,12 @@ paged_mixed_kernel(PagedParams p) {
   __shared__ __attribute__((aligned(1024))) char smem[std::max(Lds<D, NW>::NARROW, Lds<D, NW>::WIDE)];
   const int hk = blockIdx.x % p.Hkv, n = blockIdx.x / p.Hkv;
   const Division d = divide<true>(p, threadIdx.x & 63);
-  if (n < p.narrow_wgs) {
+  if (n < d.narrow) {
     narrow_stretch<T, D, NW, true, SOFTCAP>(d, smem, hk, n);
     return;
   }
   Unit u;
-  if (wide_unit_of(p, d, n - p.narrow_wgs, u)) wide_unit<T, D, NW, KG, OCC, SOFTCAP>(u, smem, hk);
+  if (wide_unit_of(p, d, n - d.narrow, u)) wide_unit<T, D, NW, KG, OCC, SOFTCAP>(u, smem, hk);
 }
 
 // Joins the partials of rows: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, lse = (M + log2 L) ln 2, with those

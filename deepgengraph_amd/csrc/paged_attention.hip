@@ -10,7 +10,8 @@ using dgg_paged::PagedParams;
 
 // The host's part of the division.
 struct HostPlan {
-  int log2_r, wide_target, wide_units, wide_slots, wide_rows, narrow_wgs, narrow_slots, narrow_rows, prefix_wide;
+  int log2_r, places, wide_target, wide_units, wide_slots, wide_rows, narrow_wgs, narrow_most, narrow_slots, narrow_rows,
+      prefix_wide;
   int64_t floats(int64_t Hkv, int64_t D) const {
     return ((int64_t)wide_slots * wide_rows + (int64_t)narrow_slots * narrow_rows) * Hkv * (D + 2);
   }
@@ -25,8 +26,8 @@ struct HostPlan {
 // chunks of up to 1,024 tokens 148, 147, 147, 158; the prefix of 16,384 133, 106, 101, 100). Narrow stretches: one
 // for each resident workgroup, of at most two per CU (32 x 16 heads of 64, up to 4,000 keys: 512 stretches 53, 768
 // 56). Beside wide units one per CU: that many saturate the memory, and more only lengthen the latency that the wide
-// units see (the step of 28 decode rows and 4 chunks at 128, 256, 384 stretches 129, 127, 132, 64 decode rows behind
-// a prefix of 8,192 77, 55, 55).
+// units see (the step of 28 decode rows and 4 chunks at 128, 256, 384 stretches 129, 127, 132). Where no sequence is
+// wide, which the lengths tell, the device divides the places anew (divide() in paged.h).
 HostPlan host_plan(int64_t B, int64_t T, bool ragged, int64_t Hq, int64_t Hkv, int64_t D, int64_t P) {
   HostPlan h{};
   const int64_t G = Hq / Hkv, Sq = T / B, CUs = 256;
@@ -40,6 +41,7 @@ HostPlan host_plan(int64_t B, int64_t T, bool ragged, int64_t Hq, int64_t Hkv, i
     const bool large = D == 128 && !ragged && T * G / 256 * Hkv >= CUs;
     h.log2_r = typical <= 64 ? 6 : large ? 8 : 7;
     h.wide_target = (int)std::max<int64_t>(1, (large ? CUs : CUs * per_cu * 7 / 8) / Hkv);
+    h.places = (int)std::max<int64_t>(2, CUs * (large ? 1 : per_cu) / Hkv);
     const int64_t R = 1ll << h.log2_r;
     // ragged: a sequence's rows fill row groups but for its last; only sequences of more than 32 rows count
     const int64_t nrg = ragged ? T * G / R + std::min(B, T * G / (dgg_paged::kNarrowRows + 1))
@@ -50,9 +52,9 @@ HostPlan host_plan(int64_t B, int64_t T, bool ragged, int64_t Hq, int64_t Hkv, i
     h.wide_rows = (int)std::min<int64_t>(R, h.prefix_wide ? T * G : most);
   }
   if (narrow) {
-    const int64_t wgs = wide ? std::min(CUs, CUs * per_cu * 3 / 4) : CUs * std::min<int64_t>(per_cu, 2);
-    h.narrow_wgs = (int)std::max<int64_t>(1, wgs / Hkv);
-    h.narrow_slots = (int)(h.narrow_wgs + B + 1);
+    h.narrow_most = (int)std::max<int64_t>(1, CUs * std::min<int64_t>(per_cu, 2) / Hkv);
+    h.narrow_wgs = wide ? (int)std::max<int64_t>(1, std::min(CUs, CUs * per_cu * 3 / 4) / Hkv) : h.narrow_most;
+    h.narrow_slots = (int)(h.narrow_most + B + 1);
     h.narrow_rows = (int)std::min<int64_t>(dgg_paged::kNarrowRows, P > 0 && !h.prefix_wide ? T * G : most);
   }
   return h;
@@ -179,9 +181,11 @@ extern "C" int dgg_attn_paged(const void* q, const void* k_pages, const void* v_
   p.wide_slots = h.wide_slots;
   p.wide_rows = h.wide_rows;
   p.narrow_wgs = h.narrow_wgs;
+  p.narrow_most = h.narrow_most;
   p.narrow_slots = h.narrow_slots;
   p.narrow_rows = h.narrow_rows;
-  p.per_wide = h.wide_target > 0 ? (float)((1.0 + 1.0 / 2048) / h.wide_target) : 0.f;
+  p.wide_target = h.wide_target;
+  p.places = h.places;
   p.rows_per_merge = (int)std::max<int64_t>(1, T * p.G * Hkv / 4096);
   hipStream_t st = dgg::as_stream(stream);
   if (D == 64) dgg_paged::launch_d64(p, dtype == DGG_BF16, st);
