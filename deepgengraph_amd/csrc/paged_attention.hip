@@ -27,7 +27,8 @@ struct HostPlan {
 // for each resident workgroup, of at most two per CU (32 x 16 heads of 64, up to 4,000 keys: 512 stretches 53, 768
 // 56). Beside wide units one per CU: that many saturate the memory, and more only lengthen the latency that the wide
 // units see (the step of 28 decode rows and 4 chunks at 128, 256, 384 stretches 129, 127, 132). Where no sequence is
-// wide, which the lengths tell, the device divides the places anew (divide() in paged.h).
+// wide, which the lengths tell, the device divides the places anew (divide() in paged.h); the grid has room for them:
+// places <= wide_target + narrow_wgs for every number of heads.
 HostPlan host_plan(int64_t B, int64_t T, bool ragged, int64_t Hq, int64_t Hkv, int64_t D, int64_t P) {
   HostPlan h{};
   const int64_t G = Hq / Hkv, Sq = T / B, CUs = 256;

@@ -200,6 +200,20 @@ def test_prefix_with_many_sequences(gpu):
     _run(gpu, [96 + b % 40 for b in range(130)], [b % 3 for b in range(130)], prefix=96, Hq=2, Hkv=2, D=64)
 
 
+@pytest.mark.parametrize("D,heads", [(64, (48, 48)), (128, (160, 160)), (128, (8, 2)), (256, (32, 16))])
+@pytest.mark.parametrize("P,more,kw", [(1024, [1, 2, 17], {}), (16, [500, 3, 700], {}), (512, [200, 300, 400], dict(window=90)),
+                                       (512, [0, 0, 5], dict(window=600))])
+def test_prefix_and_decode_rows(gpu, D, heads, P, more, kw):
+    # nearly all keys in the prefix, nearly none, a prefix that no window reaches, sequences that hold nothing else; up
+    # to as many heads as workgroups that are resident at once
+    B = 34 if heads[0] == heads[1] else 18
+    kv = [P + more[b % 3] for b in range(B)]
+    _run(gpu, kv, [1] * B, Hq=heads[0], Hkv=heads[1], D=D, prefix=P, seed=D + P, **kw)
+    if heads[0] > 100:
+        return  # (the oracle takes its time)
+    _run(gpu, kv, [1, 0] + [1] * (B - 2), Hq=heads[0], Hkv=heads[1], D=D, prefix=P, seed=D + P, tail=3, **kw)
+
+
 def test_prefix_is_the_first_sequences(gpu):
     # the other rows of the table are not looked at inside the prefix
     g = _gen(5)
